@@ -1,0 +1,424 @@
+// attn_paged.hip -- attention of one new token a sequence over keys and values in pages, and the write of new rows
+// into the pages (include/spmm_attn.h).
+//
+// Each visible key and value is read once from memory and used by the query heads of its group, so bytes bound the
+// kernel and it is laid out for loads that go straight into the matrix instructions, with no LDS on the way:
+//  - a wave takes 16 keys at a time; S^T = K Q^T (16 keys x up to 16 heads) has a lane's 16-byte piece of one key's row
+//    as its first operand;
+//  - S^T leaves a lane with keys 4 (l / 16) + r, r = 0..3, of head l % 16.  exp(S^T) register r is then, as it stands, the
+//    first operand of a 16x16x4 product in 32-bit floats over the keys {r, 4 + r, 8 + r, 12 + r}, whose second operand is
+//    value row 4 (l / 16) + r: lane l % 16 loads 16 bytes of that row and gives one element to each of 8 products.
+//    The 32-bit instruction costs 8 times a 16-bit one and is still under the time of the loads; in return the
+//    weights are not rounded and the values need no transposition.
+// A block's four waves share a stretch of the keys and join through LDS; when there are few sequences the keys are
+// split over several blocks, and a second kernel joins their parts in order.
+#include "attn_common.hpp"
+
+namespace attn {
+
+constexpr int PW = 4;                        // waves of a block
+constexpr int PK = 16;                       // keys a wave takes at a time
+constexpr int SPLIT_MIN = 256;               // keys a block takes at least
+
+struct PagedArgs {
+    Rows q, out;
+    const char *k, *v;
+    int64_t pages, page_rows, k_page, k_row, k_head, v_page, v_row, v_head, table_cols, table_stride;
+    const int32_t *table, *lengths;
+    bool k_wide, v_wide;
+    int64_t batch, limit;                    // limit: longest sequence allowed
+    int heads, kv_heads, dim, window, sinks, splits;
+    float scale2;
+    float *lse, *part;                       // part: [batch][heads][splits][dim + 2]: max, sum, weighted values
+};
+
+// The 16-key tiles that hold visible keys: `first` tiles from position 0, then those from `start` on.
+struct Span {
+    int first, start, tiles;
+    __device__ __forceinline__ int at(int i) const { return (i < first ? i : start + i - first) * PK; }
+};
+__device__ __forceinline__ Span span_of(int len, int window, int sinks) {
+    Span s;
+    const int lo = window && len > window ? len - window : 0;
+    s.start = lo / PK;
+    s.first = min((min(sinks, len) + PK - 1) / PK, s.start);
+    s.tiles = s.first + (len + PK - 1) / PK - s.start;
+    return s;
+}
+
+// V elements a lane owns: VE = dim rounded up to 16 VE; value column of lane n, element j is n * VE + j.
+template <typename T, int VE> struct VRow {
+    float x[VE];
+    __device__ __forceinline__ void load(const T *row, int n, int dim, bool wide) {
+        const int e = n * VE;
+        if (!row || e >= dim) {
+#pragma unroll
+            for (int j = 0; j < VE; ++j) x[j] = 0.f;
+            return;
+        }
+        if (wide && e + VE <= dim) {
+            typedef T vec __attribute__((ext_vector_type(VE)));
+            const vec w = *reinterpret_cast<const vec *>(row + e);
+#pragma unroll
+            for (int j = 0; j < VE; ++j) x[j] = (float)w[j];
+        } else {
+#pragma unroll
+            for (int j = 0; j < VE; ++j) x[j] = e + j < dim ? (float)row[e + j] : 0.f;
+        }
+    }
+};
+
+template <typename T, int DP>
+__global__ __launch_bounds__(PW * 64) void paged_kernel(PagedArgs A) {
+    constexpr int NS = DP / 32, VE = DP / 16;
+    const int group = A.heads / A.kv_heads, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, h4 = lane >> 4;
+    const int hb = (group + 15) / 16;                       // blocks of 16 query heads of a group
+    int id = (int)blockIdx.x;
+    const int kv = id % A.kv_heads; id /= A.kv_heads;
+    const int g0 = id % hb * 16; id /= hb;
+    const int split = id % A.splits;
+    const int64_t b = id / A.splits;
+
+    int len = A.lengths[b];
+    bool bad = len < 0 || len > A.limit;
+    if (bad) len = 0;
+    const Span sp = span_of(len, A.window, A.sinks);
+    const int per = (sp.tiles + A.splits - 1) / A.splits, t0 = split * per, t1 = min(t0 + per, sp.tiles);
+
+    const int head = kv * group + g0 + n;
+    const bool mine = g0 + n < group;
+    frag<T> qf[NS];
+    {
+        const T *qr = mine ? (const T *)A.q.ptr + b * A.q.seq + head * A.q.head : nullptr;
+#pragma unroll
+        for (int s = 0; s < NS; ++s) qf[s] = load_frag<T>(qr, s * 32 + h4 * 8, A.dim, A.q.wide);
+    }
+    const T *kb = (const T *)A.k + kv * A.k_head, *vb = (const T *)A.v + kv * A.v_head;
+    const int32_t *table = A.table + b * A.table_stride;
+
+    f32x4 o[VE];
+#pragma unroll
+    for (int j = 0; j < VE; ++j) o[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    float m = -INFINITY, sum = 0.f;
+    for (int t = t0 + wave; t < t1; t += PW) {
+        const int j0 = sp.at(t);
+        auto seen = [&](int j) { return j < len && (A.window == 0 || len - 1 - j < A.window || j < A.sinks); };
+        // row of position j in the pages, -1 if it is not seen
+        auto find = [&](int j) -> int64_t {
+            if (!seen(j)) return -1;
+            const int64_t pg = table[j / A.page_rows];
+            if (pg < 0 || pg >= A.pages) { bad = true; return -1; }
+            return pg;
+        };
+        const int jk = j0 + n;
+        const int64_t pk = find(jk);
+        const T *kr = pk < 0 ? nullptr : kb + pk * A.k_page + (jk % A.page_rows) * A.k_row;
+        f32x4 sc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = 0; s < NS; ++s) sc = mma16(load_frag<T>(kr, s * 32 + h4 * 8, A.dim, A.k_wide), qf[s], sc);
+        VRow<T, VE> vr[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int j = j0 + 4 * h4 + r;
+            const int64_t pv = find(j);
+            vr[r].load(pv < 0 ? nullptr : vb + pv * A.v_page + (j % A.page_rows) * A.v_row, n, A.dim, A.v_wide);
+        }
+        float mx = m;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            sc[r] = seen(j0 + 4 * h4 + r) ? sc[r] * A.scale2 : -INFINITY;
+            mx = fmaxf(mx, sc[r]);
+        }
+        mx = fmaxf(mx, __shfl_xor(mx, 16));
+        mx = fmaxf(mx, __shfl_xor(mx, 32));
+        const float base = mx == -INFINITY ? 0.f : mx;
+        if (__any(mx != m)) {
+            const float alpha = __builtin_amdgcn_exp2f(m - base);
+            sum *= alpha;
+            f32x4 a4;                                       // accumulator rows are heads 4 h4 + r
+#pragma unroll
+            for (int r = 0; r < 4; ++r) a4[r] = __shfl(alpha, 4 * h4 + r);
+#pragma unroll
+            for (int j = 0; j < VE; ++j) o[j] *= a4;
+            m = mx;
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            sc[r] = __builtin_amdgcn_exp2f(sc[r] - base);
+            sum += sc[r];
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int j = 0; j < VE; ++j) o[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(sc[r], vr[r].x[j], o[j], 0, 0, 0);
+    }
+    sum += __shfl_xor(sum, 16);
+    sum += __shfl_xor(sum, 32);
+    if (__any(bad)) sum = __builtin_nanf("");
+
+    // join the waves: in wave order
+    __shared__ float sm[PW][16], ss[PW][16];
+    __shared__ float so[PW][16][DP + 4];
+    if (h4 == 0) {
+        sm[wave][n] = m;
+        ss[wave][n] = sum;
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int j = 0; j < VE; ++j) so[wave][4 * h4 + r][n * VE + j] = o[j][r];
+    __syncthreads();
+    for (int i = threadIdx.x; i < 16 * DP; i += PW * 64) {
+        const int hh = i / DP, d = i % DP;
+        if (g0 + hh >= group || d >= A.dim) continue;
+        float mx = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < PW; ++w) mx = fmaxf(mx, sm[w][hh]);
+        const float base = mx == -INFINITY ? 0.f : mx;
+        float tot = 0.f, acc = 0.f;
+#pragma unroll
+        for (int w = 0; w < PW; ++w) {
+            const float f = __builtin_amdgcn_exp2f(sm[w][hh] - base);
+            tot += f * ss[w][hh];
+            acc += f * so[w][hh][d];
+        }
+        const int hd = kv * group + g0 + hh;
+        if (A.splits == 1) {
+            ((T *)A.out.ptr)[b * A.out.seq + hd * A.out.head + d] = narrow<T>(tot == 0.f ? 0.f : acc / tot);
+            if (d == 0) A.lse[b * A.heads + hd] = tot == 0.f ? -INFINITY : mx * LN2 + __logf(tot);
+        } else {
+            float *p = A.part + ((b * A.heads + hd) * A.splits + split) * (A.dim + 2);
+            if (d == 0) {
+                p[0] = mx;
+                p[1] = tot;
+            }
+            p[2 + d] = acc;
+        }
+    }
+}
+
+// One wave a (sequence, head): its parts joined in order.
+template <typename T> __global__ __launch_bounds__(64) void paged_join_kernel(PagedArgs A) {
+    const int64_t x = blockIdx.x, b = x / A.heads;
+    const int hd = (int)(x % A.heads), lane = threadIdx.x;
+    const float *p = A.part + x * A.splits * (A.dim + 2);
+    float mx = -INFINITY;
+    for (int s = 0; s < A.splits; ++s) mx = fmaxf(mx, p[s * (A.dim + 2)]);
+    const float base = mx == -INFINITY ? 0.f : mx;
+    float tot = 0.f, a0 = 0.f, a1 = 0.f;
+    for (int s = 0; s < A.splits; ++s) {
+        const float *ps = p + s * (A.dim + 2);
+        const float f = __builtin_amdgcn_exp2f(ps[0] - base);
+        tot += f * ps[1];
+        if (lane < A.dim) a0 += f * ps[2 + lane];
+        if (lane + 64 < A.dim) a1 += f * ps[2 + lane + 64];
+    }
+    const float inv = tot == 0.f ? 0.f : 1.f / tot;
+    T *dst = (T *)A.out.ptr + b * A.out.seq + hd * A.out.head;
+    if (lane < A.dim) dst[lane] = narrow<T>(a0 * inv);
+    if (lane + 64 < A.dim) dst[lane + 64] = narrow<T>(a1 * inv);
+    if (lane == 0) A.lse[x] = tot == 0.f ? -INFINITY : mx * LN2 + __logf(tot);
+}
+
+// ------------------------------------------------------------------------------------------------ append
+struct AppendArgs {
+    Rows k, v;
+    char *kp, *vp;
+    const int32_t *cu;
+    int64_t pages, page_rows, k_page, k_row, k_head, v_page, v_row, v_head, table_cols, table_stride;
+    const int32_t *table, *lengths;
+    int64_t batch, rows, es;
+    int kv_heads, dim;
+    bool k_wide, v_wide;
+};
+
+// 16 lanes a (row, head): it is moved whole, by 16-byte pieces where everything is aligned to them.
+__global__ __launch_bounds__(256) void append_kernel(AppendArgs A) {
+    const int64_t x = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
+    if (x >= A.rows * A.kv_heads) return;
+    const int64_t row = x / A.kv_heads;
+    const int head = (int)(x % A.kv_heads), l = threadIdx.x & 15;
+    int64_t b = row, pos;
+    if (A.cu) {
+        int64_t lo = 0, hi = A.batch;                        // last sequence that starts at or before the row
+        while (hi - lo > 1) {
+            const int64_t mid = (lo + hi) / 2;
+            if (A.cu[mid] <= row) lo = mid; else hi = mid;
+        }
+        b = lo;
+        if (row < A.cu[b] || row >= A.cu[b + 1]) return;     // behind the last sequence
+        pos = (int64_t)A.lengths[b] - A.cu[b + 1] + row;
+    } else {
+        pos = (int64_t)A.lengths[b] - 1;
+    }
+    if (pos < 0 || A.lengths[b] > A.table_cols * A.page_rows) return;
+    const int64_t pg = A.table[b * A.table_stride + pos / A.page_rows];
+    if (pg < 0 || pg >= A.pages) return;
+    const int64_t slot = pos % A.page_rows;
+    const char *ks = A.k.ptr + (row * A.k.row + head * A.k.head) * A.es, *vs = A.v.ptr + (row * A.v.row + head * A.v.head) * A.es;
+    char *kd = A.kp + (pg * A.k_page + slot * A.k_row + head * A.k_head) * A.es;
+    char *vd = A.vp + (pg * A.v_page + slot * A.v_row + head * A.v_head) * A.es;
+    const int bytes = A.dim * (int)A.es;
+    auto move = [&](char *d, const char *s, bool wide) {
+        if (wide)
+            for (int i = l * 16; i < bytes; i += 256) *(uint4 *)(d + i) = *(const uint4 *)(s + i);
+        else
+            for (int i = l * 2; i < bytes; i += 32) *(uint16_t *)(d + i) = *(const uint16_t *)(s + i);
+    };
+    move(kd, ks, A.k_wide);
+    move(vd, vs, A.v_wide);
+}
+
+// ------------------------------------------------------------------------------------------------ host
+static int check_pages(const spmm_attn_desc_t *a, const spmm_attn_pages_t *p, const char *where, bool written, bool *k_wide,
+                       bool *v_wide) {
+    if (!p) return fail(SPMM_HIP_ERR_ARG, "%s: no pages", where);
+    if (p->pages < 0 || p->page_rows < 1 || p->table_cols < 0 || p->table_stride < 0)
+        return fail(SPMM_HIP_ERR_ARG, "%s: %lld pages of %lld rows, %lld table columns", where, (long long)p->pages,
+                    (long long)p->page_rows, (long long)p->table_cols);
+    if (p->pages > INT32_MAX || p->page_rows > INT32_MAX / 2 || p->table_cols > (INT64_C(1) << 40))
+        return fail(SPMM_HIP_ERR_OVERFLOW, "%s: sizes of the pages", where);
+    if (a->batch > 1 && p->table_stride < p->table_cols && p->table_stride != 0)
+        return fail(SPMM_HIP_ERR_ARG, "%s: the table's rows overlap", where);
+    if (a->batch > 0 && (!p->lengths || (p->table_cols > 0 && !p->table) || (p->pages > 0 && (!p->k || !p->v))))
+        return fail(SPMM_HIP_ERR_ARG, "%s: pages, table or lengths are NULL", where);
+    if (((uintptr_t)p->table | (uintptr_t)p->lengths) % 4) return fail(SPMM_HIP_ERR_ARG, "%s: table or lengths are not aligned", where);
+    // the same rules as for rows: (page, row, head) stand for (sequence, row, head)
+    const spmm_attn_rows_t k = {p->k, p->k_page, p->k_row, p->k_head}, v = {p->v, p->v_page, p->v_row, p->v_head};
+    Rows r;
+    int st = check_rows(a, &k, where, "the key pages", p->pages, p->page_rows, a->kv_heads, written, &r);
+    if (st == SPMM_HIP_OK) st = check_rows(a, &v, where, "the value pages", p->pages, p->page_rows, a->kv_heads, written, &r);
+    if (st != SPMM_HIP_OK) return st;
+    const int64_t el = 16 / (int64_t)elem_size(a->dtype);
+    auto wide = [&](const void *ptr, int64_t s0, int64_t s1, int64_t s2) {
+        return (uintptr_t)ptr % 16 == 0 && s0 % el == 0 && s1 % el == 0 && s2 % el == 0 && a->dim % el == 0;
+    };
+    *k_wide = wide(p->k, p->k_page, p->k_row, p->k_head);
+    *v_wide = wide(p->v, p->v_page, p->v_row, p->v_head);
+    return SPMM_HIP_OK;
+}
+
+// Blocks that share a sequence's keys: enough for four blocks a compute unit in all, each with SPLIT_MIN keys or more.
+static int64_t split_count(const spmm_attn_desc_t *a, int64_t max_length) {
+    const int64_t group = a->heads / a->kv_heads, base = a->batch * a->kv_heads * ((group + 15) / 16);
+    int64_t keys = max_length;
+    if (a->window && a->window < keys) keys = (int64_t)a->window + (a->sinks < keys - a->window ? a->sinks : keys - a->window);
+    const int64_t most = (keys + SPLIT_MIN - 1) / SPLIT_MIN, want = base > 0 ? (1024 + base - 1) / base : 1;
+    const int64_t n = want < most ? want : most;
+    return n < 1 ? 1 : n;
+}
+
+template <typename T> static const void *paged_of(int dim) {
+    return dim <= 64 ? (const void *)paged_kernel<T, 64> : (const void *)paged_kernel<T, 128>;
+}
+
+}  // namespace attn
+
+using namespace attn;
+
+extern "C" int spmm_attn_paged_work(const spmm_attn_desc_t *a, int64_t max_length, size_t *bytes) {
+    const int st = check_desc(a, "attn_paged_work");
+    if (st != SPMM_HIP_OK) return st;
+    if (!bytes || max_length < 0 || max_length > INT32_MAX / 2)
+        return fail(SPMM_HIP_ERR_ARG, "attn_paged_work: bytes is NULL, or max_length %lld", (long long)max_length);
+    const int64_t s = split_count(a, max_length);
+    *bytes = s > 1 ? (size_t)(a->batch * a->heads * s * (a->dim + 2)) * 4 : 0;
+    return SPMM_HIP_OK;
+}
+
+extern "C" int spmm_attn_paged(const spmm_attn_desc_t *a, const spmm_attn_rows_t *q, const spmm_attn_pages_t *pages,
+                               int64_t max_length, const spmm_attn_rows_t *out, float *lse, void *work, size_t work_bytes,
+                               void *stream) {
+    const char *W = "attn_paged";
+    PagedArgs A = {};
+    int st = check_desc(a, W);
+    if (st != SPMM_HIP_OK) return st;
+    if ((st = check_rows(a, q, W, "q", a->batch, 1, a->heads, false, &A.q)) ||
+        (st = check_rows(a, out, W, "out", a->batch, 1, a->heads, true, &A.out)) ||
+        (st = check_pages(a, pages, W, false, &A.k_wide, &A.v_wide)))
+        return st;
+    size_t need = 0;
+    if ((st = spmm_attn_paged_work(a, max_length, &need))) return st;
+    if (a->batch == 0) return SPMM_HIP_OK;
+    if (!lse || (uintptr_t)lse % 4) return fail(SPMM_HIP_ERR_ARG, "%s: lse is NULL or not aligned", W);
+    if (need > 0 && (!work || (uintptr_t)work % 16 || work_bytes < need))
+        return fail(SPMM_HIP_ERR_ARG, "%s: the workspace needs %zu bytes, 16-byte aligned", W, need);
+    A.k = (const char *)pages->k;
+    A.v = (const char *)pages->v;
+    A.pages = pages->pages;
+    A.page_rows = pages->page_rows;
+    A.k_page = pages->k_page;
+    A.k_row = pages->k_row;
+    A.k_head = pages->k_head;
+    A.v_page = pages->v_page;
+    A.v_row = pages->v_row;
+    A.v_head = pages->v_head;
+    A.table = pages->table;
+    A.lengths = pages->lengths;
+    A.table_cols = pages->table_cols;
+    A.table_stride = pages->table_stride;
+    A.batch = a->batch;
+    A.limit = pages->table_cols > max_length / pages->page_rows ? max_length : pages->table_cols * pages->page_rows;
+    A.heads = a->heads;
+    A.kv_heads = a->kv_heads;
+    A.dim = a->dim;
+    A.window = a->window;
+    A.sinks = a->window ? a->sinks : 0;
+    A.splits = (int)split_count(a, max_length);
+    A.scale2 = a->scale * LOG2E;
+    A.lse = lse;
+    A.part = (float *)work;
+    OnDevice on(a->device, W);
+    if (on.status) return on.status;
+    const void *kern = a->dtype == SPMM_ATTN_F32 ? paged_of<float>(a->dim)
+                       : a->dtype == SPMM_ATTN_F16 ? paged_of<_Float16>(a->dim) : paged_of<__bf16>(a->dim);
+    const void *join = a->dtype == SPMM_ATTN_F32 ? (const void *)paged_join_kernel<float>
+                       : a->dtype == SPMM_ATTN_F16 ? (const void *)paged_join_kernel<_Float16>
+                                                   : (const void *)paged_join_kernel<__bf16>;
+    void *args[] = {&A};
+    const int64_t hb = (a->heads / a->kv_heads + 15) / 16;
+    if ((st = launch(kern, W, a->batch * A.splits * hb * a->kv_heads, PW * 64, args, stream))) return st;
+    return A.splits > 1 ? launch(join, W, a->batch * a->heads, 64, args, stream) : SPMM_HIP_OK;
+}
+
+extern "C" int spmm_attn_append(const spmm_attn_desc_t *a, const spmm_attn_rows_t *k, const spmm_attn_rows_t *v,
+                                const int32_t *cu, const spmm_attn_pages_t *pages, void *stream) {
+    const char *W = "attn_append";
+    AppendArgs A = {};
+    int st = check_desc(a, W);
+    if (st != SPMM_HIP_OK) return st;
+    if ((uintptr_t)cu % 4) return fail(SPMM_HIP_ERR_ARG, "%s: offsets are not aligned", W);
+    const int64_t rows = cu ? a->q_len : a->batch;
+    bool kw, vw;
+    if ((st = check_rows(a, k, W, "k", 1, rows, a->kv_heads, false, &A.k)) ||
+        (st = check_rows(a, v, W, "v", 1, rows, a->kv_heads, false, &A.v)) ||
+        (st = check_pages(a, pages, W, true, &kw, &vw)))
+        return st;
+    if (rows == 0 || a->batch == 0 || pages->pages == 0) return SPMM_HIP_OK;
+    A.k_wide = A.k.wide && kw;
+    A.v_wide = A.v.wide && vw;
+    A.kp = (char *)pages->k;
+    A.vp = (char *)pages->v;
+    A.cu = cu;
+    A.pages = pages->pages;
+    A.page_rows = pages->page_rows;
+    A.k_page = pages->k_page;
+    A.k_row = pages->k_row;
+    A.k_head = pages->k_head;
+    A.v_page = pages->v_page;
+    A.v_row = pages->v_row;
+    A.v_head = pages->v_head;
+    A.table = pages->table;
+    A.lengths = pages->lengths;
+    A.table_cols = pages->table_cols;
+    A.table_stride = pages->table_stride;
+    A.batch = a->batch;
+    A.rows = rows;
+    A.es = (int64_t)elem_size(a->dtype);
+    A.kv_heads = a->kv_heads;
+    A.dim = a->dim;
+    OnDevice on(a->device, W);
+    if (on.status) return on.status;
+    void *args[] = {&A};
+    return launch((const void *)append_kernel, W, (rows * a->kv_heads + 15) / 16, 256, args, stream);
+}

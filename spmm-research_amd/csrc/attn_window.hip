@@ -1,0 +1,221 @@
+// attn_window.hip -- causal attention under a sliding window with first keys that stay visible (include/spmm_attn.h).
+//
+// One pass over the keys with a running maximum and sum.  A workgroup has four waves of 32 queries each of one head; the
+// keys and values that its 128 queries see come by tiles through LDS.  Scores are formed transposed, S^T = K Q^T, so a
+// lane owns one query (column l % 32) and half of the tile's keys: the softmax statistics of a query need one exchange
+// between two lanes, and S^T leaves the matrix unit in the layout in which exp(S^T) is the second operand of
+// O^T = V^T P^T -- the weights never pass through LDS.  V^T comes from the row-major tile by the transposing LDS read.
+#include "attn_window.hpp"
+
+namespace attn {
+
+template <typename T> constexpr int BN_OF = sizeof(T) == 2 ? 64 : 32;      // keys of a tile
+constexpr int BM = 128;                                                      // queries of a workgroup
+
+template <typename T, int DP>
+__global__ __launch_bounds__(256, 2) void window_kernel(WindowArgs A) {
+    using L = Tile<T, DP>;
+    constexpr int BN = BN_OF<T>, ND = DP / 32, NS = DP / 16, NK = BN / 32;
+    __shared__ __align__(16) T sk[2][BN * L::PITCH];
+    __shared__ __align__(16) T sv[2][BN * L::PITCH];
+    __shared__ int odd;                              // some staged value of a partly visible tile was not finite
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
+    int kv, g, t;
+    place(A, A.heads / A.kv_heads, &kv, &g, &t);
+    t = A.tiles - 1 - t;                             // late queries see more keys: they start first
+    const int head = kv * (A.heads / A.kv_heads) + g;
+    const bool packed = A.cu_q != nullptr;
+    const Seq s = find_tile(t, BM, false, A.cu_q, A.cu_k, A.batch, A.q_len, A.k_len);
+    if (s.tile < 0) {
+        if (A.zero_rest && packed) {
+            const int64_t from = s.rest + (int64_t)(t - s.nq) * BM, step = (int64_t)(A.tiles - s.nq) * BM;
+            zero_rows<T>(A.out, from, step, BM, A.q_len, head, A.dim);
+            for (int64_t c = from; c < A.q_len; c += step)
+                for (int64_t r = c + tid; r < c + BM && r < A.q_len; r += blockDim.x) A.lse[r * A.heads + head] = -INFINITY;
+        }
+        return;
+    }
+    if (tid == 0) odd = 0;
+
+    const int shift = s.nk - s.nq, m0 = s.tile * BM, m1 = min(m0 + BM, s.nq) - 1;
+    const int pmin = m0 + shift, pmax = m1 + shift;                       // positions of the block's queries
+    const int lo = A.mask.window ? max(0, pmin - A.mask.window + 1) : 0;  // first key that the window holds
+    const int lt = lo / BN, ht = pmax >= 0 ? pmax / BN : -1;
+    const int ns = pmax >= 0 ? min((min(A.mask.sinks, pmax + 1) + BN - 1) / BN, lt) : 0;      // tiles of first keys before
+    const int tiles = ns + max(0, ht - lt + 1);
+    auto tile_at = [&](int i) { return (i < ns ? i : lt + i - ns) * BN; };
+
+    const T *kb = seq_base<T>(A.k, s, s.k0, packed, kv), *vb = seq_base<T>(A.v, s, s.k0, packed, kv);
+    const int i = m0 + wave * 32 + (lane & 31), p = i + shift;            // this lane's query
+    const bool mine = i < s.nq;
+    const int w0 = m0 + wave * 32 + shift, w1 = min(w0 + 31, pmax);       // the wave's positions
+    frag<T> qf[NS];
+    {
+        const T *qr = mine ? seq_base<T>(A.q, s, s.q0, packed, head) + i * A.q.row : nullptr;
+#pragma unroll
+        for (int st = 0; st < NS; ++st) qf[st] = load_frag<T>(qr, st * 16 + h * 8, A.dim, A.q.wide);
+    }
+
+    Stage<T, DP, BN, 256> ks, vs;
+    auto stage_load = [&](int j0) {
+        // keys that no query of the block sees are not read: they may be anything
+        auto live = [&](int r) { const int j = j0 + r; return j <= pmax && (j >= lo || j < A.mask.sinks); };
+        ks.load(tid, A.dim, A.k.wide, [&](int r) { return live(r) ? kb + (int64_t)(j0 + r) * A.k.row : nullptr; });
+        vs.load(tid, A.dim, A.v.wide, [&](int r) { return live(r) ? vb + (int64_t)(j0 + r) * A.v.row : nullptr; });
+    };
+    auto stage_store = [&](int j0, int buf) {
+        if (!A.mask.all(pmin, pmax, j0, j0 + BN - 1) && vs.any_not_finite()) odd = 1;
+        ks.store(tid, sk[buf]);
+        vs.store(tid, sv[buf]);
+    };
+
+    f32x16 o[ND];
+#pragma unroll
+    for (int d = 0; d < ND; ++d) o[d] = zero16();
+    float m = -INFINITY, sum = 0.f;
+    __syncthreads();                                 // `odd` is set
+    if (tiles) {
+        stage_load(tile_at(0));
+        stage_store(tile_at(0), 0);
+    }
+    __syncthreads();
+    for (int it = 0; it < tiles; ++it) {
+        const int j0 = tile_at(it), buf = it & 1;
+        if (it + 1 < tiles) stage_load(tile_at(it + 1));
+        if (w0 <= w1 && A.mask.any(w0, w1, j0, j0 + BN - 1)) {
+            const bool full = A.mask.all(w0, w1, j0, j0 + BN - 1);
+            f32x16 sc[NK];
+#pragma unroll
+            for (int n = 0; n < NK; ++n) {
+                sc[n] = zero16();
+#pragma unroll
+                for (int st = 0; st < NS; ++st)
+                    sc[n] = mma32(L::row_frag(sk[buf], n * 32 + (lane & 31), st * 16 + h * 8), qf[st], sc[n]);
+            }
+            float mx = m;
+#pragma unroll
+            for (int n = 0; n < NK; ++n)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    float x = sc[n][r] * A.scale2;
+                    if (!full && !A.mask.sees(p, j0 + n * 32 + row_of(r) + 4 * h)) x = -INFINITY;
+                    sc[n][r] = x;
+                    mx = fmaxf(mx, x);
+                }
+            mx = fmaxf(mx, __shfl_xor(mx, 32));
+            const float base = mx == -INFINITY ? 0.f : mx;
+            if (__any(mx != m)) {
+                const float alpha = __builtin_amdgcn_exp2f(m - base);
+                sum *= alpha;
+#pragma unroll
+                for (int d = 0; d < ND; ++d) o[d] *= alpha;
+                m = mx;
+            }
+#pragma unroll
+            for (int n = 0; n < NK; ++n)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    sc[n][r] = __builtin_amdgcn_exp2f(sc[n][r] - base);
+                    sum += sc[n][r];
+                }
+            const bool careful = !full && odd;
+#pragma unroll
+            for (int n = 0; n < NK; ++n)
+#pragma unroll
+                for (int k2 = 0; k2 < 2; ++k2) {
+                    const frag<T> pf = next_operand<T>(sc[n], k2);
+#pragma unroll
+                    for (int d = 0; d < ND; ++d) {
+                        frag<T> vf = L::col_frag(sv[buf], n * 32 + k2 * 16, d * 32, lane);
+                        if (careful) vf = only_finite<T>(vf);
+                        o[d] = mma32(vf, pf, o[d]);
+                    }
+                }
+            if (careful)
+                add_not_finite<T, DP>(o, sv[buf], BN, lane, [&](int r) { return A.mask.sees(p, j0 + r); });
+        }
+        if (it + 1 < tiles) stage_store(tile_at(it + 1), buf ^ 1);
+        __syncthreads();
+    }
+    sum += __shfl_xor(sum, 32);
+    if (!mine) return;
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    T *dst = seq_base<T>(A.out, s, s.q0, packed, head) + i * A.out.row;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; r += 4)
+            store4<T>(dst, d * 32 + row_of(r) + 4 * h, A.dim, A.out.wide,
+                      f32x4{o[d][r] * inv, o[d][r + 1] * inv, o[d][r + 2] * inv, o[d][r + 3] * inv});
+    if (h == 0) {
+        const int64_t row = packed ? s.q0 + i : s.b * A.q_len + i;
+        A.lse[row * A.heads + head] = sum == 0.f ? -INFINITY : m * LN2 + __logf(sum);
+    }
+}
+
+int window_args(const spmm_attn_desc_t *a, const char *where, const int32_t *cu_q, const int32_t *cu_k, WindowArgs *out) {
+    if (!cu_q != !cu_k) return fail(SPMM_HIP_ERR_ARG, "%s: offsets for only one of queries and keys", where);
+    if (((uintptr_t)cu_q | (uintptr_t)cu_k) % 4) return fail(SPMM_HIP_ERR_ARG, "%s: offsets are not aligned", where);
+    *out = WindowArgs{};
+    out->cu_q = cu_q;
+    out->cu_k = cu_k;
+    out->batch = a->batch;
+    out->q_len = a->q_len;
+    out->k_len = a->k_len;
+    out->heads = a->heads;
+    out->kv_heads = a->kv_heads;
+    out->dim = a->dim;
+    // a window over every key is no window; first keys beyond the last are none
+    out->mask.window = a->window >= a->k_len ? 0 : a->window;
+    out->mask.sinks = out->mask.window ? (int)(a->sinks < a->k_len ? a->sinks : a->k_len) : 0;
+    out->scale = a->scale;
+    out->scale2 = a->scale * LOG2E;
+    out->zero_rest = a->zero_rest;
+    return SPMM_HIP_OK;
+}
+
+// Tiles over all sequences: with offsets a bound that holds for any lengths of that sum, and one more, which lies behind
+// the last sequence, where rows there are to be set.
+int tile_count(const spmm_attn_desc_t *a, const char *where, bool packed, int64_t len, int rows, int *tiles) {
+    const int64_t n = packed ? len / rows + a->batch + (a->zero_rest ? 1 : 0) : a->batch * ((len + rows - 1) / rows);
+    if (n > INT32_MAX / a->heads) return fail(SPMM_HIP_ERR_OVERFLOW, "%s: too many tiles of queries or keys", where);
+    *tiles = (int)n;
+    return SPMM_HIP_OK;
+}
+
+template <typename T> static const void *window_of(int dim) {
+    return dim <= 64 ? (const void *)window_kernel<T, 64> : dim <= 96 ? (const void *)window_kernel<T, 96>
+                                                                      : (const void *)window_kernel<T, 128>;
+}
+
+}  // namespace attn
+
+using namespace attn;
+
+extern "C" int spmm_attn_window(const spmm_attn_desc_t *a, const spmm_attn_rows_t *q, const spmm_attn_rows_t *k,
+                                const spmm_attn_rows_t *v, const int32_t *cu_q, const int32_t *cu_k,
+                                const spmm_attn_rows_t *out, float *lse, void *stream) {
+    const char *W = "attn_window";
+    WindowArgs A;
+    int st = check_desc(a, W);
+    if (st == SPMM_HIP_OK) st = window_args(a, W, cu_q, cu_k, &A);
+    if (st != SPMM_HIP_OK) return st;
+    const bool packed = cu_q != nullptr;
+    const int64_t nb = packed ? 1 : a->batch;
+    if ((st = check_rows(a, q, W, "q", nb, a->q_len, a->heads, false, &A.q)) ||
+        (st = check_rows(a, k, W, "k", nb, a->k_len, a->kv_heads, false, &A.k)) ||
+        (st = check_rows(a, v, W, "v", nb, a->k_len, a->kv_heads, false, &A.v)) ||
+        (st = check_rows(a, out, W, "out", nb, a->q_len, a->heads, true, &A.out)))
+        return st;
+    if (nb == 0 || a->q_len == 0 || a->batch == 0) return SPMM_HIP_OK;
+    if (!lse || (uintptr_t)lse % 4) return fail(SPMM_HIP_ERR_ARG, "%s: lse is NULL or not aligned", W);
+    A.lse = lse;
+    if ((st = tile_count(a, W, packed, a->q_len, BM, &A.tiles))) return st;
+    OnDevice on(a->device, W);
+    if (on.status) return on.status;
+    const void *kern = a->dtype == SPMM_ATTN_F32 ? window_of<float>(a->dim)
+                       : a->dtype == SPMM_ATTN_F16 ? window_of<_Float16>(a->dim) : window_of<__bf16>(a->dim);
+    void *args[] = {&A};
+    return launch(kern, W, (int64_t)A.tiles * a->heads, 256, args, stream);
+}
