@@ -73,7 +73,6 @@ __device__ __forceinline__ bool finite_f(float x) { return fabsf(x) < INFINITY; 
 template <typename T, int DP> struct Tile {
     static constexpr int PITCH = DP <= 64 ? 64 : 128;
     static constexpr int EL = 16 / (int)sizeof(T);          // elements of a 16-byte piece
-    static constexpr int PIECES = DP / EL;                  // pieces of a row that hold something
 
     static __device__ __forceinline__ int swizzle(int row) {
         if constexpr (sizeof(T) == 2)
@@ -117,45 +116,55 @@ template <typename T, int DP> struct Tile {
     }
 };
 
-// A lane's share of a tile on its way from memory to LDS: piece `tid + i * THREADS` of the R x PIECES pieces.
-template <typename T, int DP, int R, int THREADS> struct Stage {
-    using L = Tile<T, DP>;
-    static constexpr int N = (R * L::PIECES + THREADS - 1) / THREADS;
-    uint4 w[N];
+__device__ __align__(16) const uint32_t zero_piece[4] = {0, 0, 0, 0};
 
-    // row(r): address of the tile's row r (its head's first element), or nullptr for a row of zeros.  `wide`: rows are
-    // 16-byte aligned and dim is a multiple of a piece.
-    template <typename F> __device__ __forceinline__ void load(int tid, int dim, bool wide, F row) {
+// Brings the R rows of a tile from memory to LDS, THREADS threads together.
+template <typename T, int DP, int R, int THREADS> struct Mover {
+    using L = Tile<T, DP>;
+    static constexpr int PP = L::PITCH / L::EL;             // 16-byte places of a row
+    static constexpr int N = R * PP / THREADS;
+    static_assert(R * PP % THREADS == 0 && THREADS % 64 == 0, "whole waves of pieces");
+
+    // By the loads that write LDS themselves: lane l of a wave fills place l of 64 consecutive ones, so the exchange of
+    // pieces within a row is in which piece a lane asks for; what is not there comes from a piece of zeros.  Rows are
+    // 16-byte aligned and dim is a multiple of a piece.  row(r): address of the tile's row r, nullptr for zeros.  The
+    // tile is there after arrived() and a barrier.
+    template <typename F> static __device__ __forceinline__ void send(int tid, int dim, T *tile, F row) {
+        typedef __attribute__((address_space(3))) void lds_void;
+        typedef __attribute__((address_space(1))) const void global_void;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int p = tid + i * THREADS, r = p / L::PIECES, e = (p % L::PIECES) * L::EL;
-            w[i] = make_uint4(0, 0, 0, 0);
-            if (R * L::PIECES % THREADS != 0 && p >= R * L::PIECES) continue;
+            const int p = tid + i * THREADS, r = p / PP, e = ((p % PP) ^ L::swizzle(r)) * L::EL;
             const T *src = row(r);
-            if (!src || e >= dim) continue;
-            if (wide) {
-                w[i] = *reinterpret_cast<const uint4 *>(src + e);
-            } else {
-                T tmp[L::EL];
-#pragma unroll
-                for (int j = 0; j < L::EL; ++j) tmp[j] = e + j < dim ? src[e + j] : (T)0.f;
-                __builtin_memcpy(&w[i], tmp, 16);
-            }
+            const void *from = src && e < dim ? (const void *)(src + e) : (const void *)zero_piece;
+            __builtin_amdgcn_global_load_lds((global_void *)from,
+                                             (lds_void *)(tile + (i * THREADS + (tid & ~63)) * L::EL), 16, 0, 0);
         }
     }
-    __device__ __forceinline__ void store(int tid, T *tile) const {
+    static __device__ __forceinline__ void arrived() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+    // Through registers, element by element: any alignment and width.
+    template <typename F> static __device__ __forceinline__ void copy(int tid, int dim, T *tile, F row) {
+#pragma unroll 1
+        for (int p = tid; p < R * PP; p += THREADS) {
+            const int r = p / PP, e = ((p % PP) ^ L::swizzle(r)) * L::EL;
+            const T *src = row(r);
+            T tmp[L::EL];
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int p = tid + i * THREADS;
-            if (R * L::PIECES % THREADS != 0 && p >= R * L::PIECES) continue;
-            *reinterpret_cast<uint4 *>(tile + L::at(p / L::PIECES, (p % L::PIECES) * L::EL)) = w[i];
+            for (int j = 0; j < L::EL; ++j) tmp[j] = src && e + j < dim ? src[e + j] : (T)0.f;
+            uint4 w;
+            __builtin_memcpy(&w, tmp, 16);
+            *reinterpret_cast<uint4 *>(tile + p * L::EL) = w;
         }
     }
-    __device__ __forceinline__ bool any_not_finite() const {
+    // Of the pieces that this thread brought (arrived, or copied).
+    static __device__ __forceinline__ bool any_not_finite(int tid, const T *tile) {
         uint32_t b = 0;
 #pragma unroll
-        for (int i = 0; i < N; ++i)
-            b |= not_finite<T>(w[i].x) | not_finite<T>(w[i].y) | not_finite<T>(w[i].z) | not_finite<T>(w[i].w);
+        for (int i = 0; i < N; ++i) {
+            const uint4 w = *reinterpret_cast<const uint4 *>(tile + (tid + i * THREADS) * L::EL);
+            b |= not_finite<T>(w.x) | not_finite<T>(w.y) | not_finite<T>(w.z) | not_finite<T>(w.w);
+        }
         return b != 0;
     }
 };

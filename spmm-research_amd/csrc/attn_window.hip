@@ -54,35 +54,47 @@ __global__ __launch_bounds__(256, 2) void window_kernel(WindowArgs A) {
     {
         const T *qr = mine ? seq_base<T>(A.q, s, s.q0, packed, head) + i * A.q.row : nullptr;
 #pragma unroll
-        for (int st = 0; st < NS; ++st) qf[st] = load_frag<T>(qr, st * 16 + h * 8, A.dim, A.q.wide);
+        for (int st = 0; st < NS; ++st) {
+            qf[st] = load_frag<T>(qr, st * 16 + h * 8, A.dim, A.q.wide);
+            // the largest score is then the largest product, and a masked product of -inf stays one
+            if (A.scale2 < 0.f) qf[st] = -qf[st];
+            if (A.scale2 == 0.f) qf[st] = frag<T>{};
+        }
     }
+    const float scale2 = A.scale2 == 0.f ? 1.f : fabsf(A.scale2);
 
-    Stage<T, DP, BN, 256> ks, vs;
-    auto stage_load = [&](int j0) {
-        // keys that no query of the block sees are not read: they may be anything
-        auto live = [&](int r) { const int j = j0 + r; return j <= pmax && (j >= lo || j < A.mask.sinks); };
-        ks.load(tid, A.dim, A.k.wide, [&](int r) { return live(r) ? kb + (int64_t)(j0 + r) * A.k.row : nullptr; });
-        vs.load(tid, A.dim, A.v.wide, [&](int r) { return live(r) ? vb + (int64_t)(j0 + r) * A.v.row : nullptr; });
+    using Move = Mover<T, DP, BN, 256>;
+    const bool direct = A.k.wide && A.v.wide;
+    // keys that no query of the block sees are not read: they may be anything
+    auto key_row = [&](const T *base, const Rows &R, int j) {
+        return j <= pmax && (j >= lo || j < A.mask.sinks) ? base + (int64_t)j * R.row : nullptr;
     };
-    auto stage_store = [&](int j0, int buf) {
-        if (!A.mask.all(pmin, pmax, j0, j0 + BN - 1) && vs.any_not_finite()) odd = 1;
-        ks.store(tid, sk[buf]);
-        vs.store(tid, sv[buf]);
+    auto bring = [&](int j0, int buf, auto how) {
+        how(sk[buf], [&](int r) { return key_row(kb, A.k, j0 + r); });
+        how(sv[buf], [&](int r) { return key_row(vb, A.v, j0 + r); });
+    };
+    auto send = [&](T *tile, auto row) { Move::send(tid, A.dim, tile, row); };
+    auto copy = [&](T *tile, auto row) { Move::copy(tid, A.dim, tile, row); };
+    // the tile is in LDS but for a barrier
+    auto settle = [&](int j0, int buf) {
+        if (direct) Move::arrived();
+        else bring(j0, buf, copy);
+        if (!A.mask.all(pmin, pmax, j0, j0 + BN - 1) && Move::any_not_finite(tid, sv[buf])) odd = 1;
     };
 
     f32x16 o[ND];
 #pragma unroll
     for (int d = 0; d < ND; ++d) o[d] = zero16();
-    float m = -INFINITY, sum = 0.f;
+    float m = -INFINITY, sum = 0.f;                  // of the scores times scale2
     __syncthreads();                                 // `odd` is set
     if (tiles) {
-        stage_load(tile_at(0));
-        stage_store(tile_at(0), 0);
+        if (direct) bring(tile_at(0), 0, send);
+        settle(tile_at(0), 0);
     }
     __syncthreads();
     for (int it = 0; it < tiles; ++it) {
         const int j0 = tile_at(it), buf = it & 1;
-        if (it + 1 < tiles) stage_load(tile_at(it + 1));
+        if (direct && it + 1 < tiles) bring(tile_at(it + 1), buf ^ 1, send);
         if (w0 <= w1 && A.mask.any(w0, w1, j0, j0 + BN - 1)) {
             const bool full = A.mask.all(w0, w1, j0, j0 + BN - 1);
             f32x16 sc[NK];
@@ -93,17 +105,20 @@ __global__ __launch_bounds__(256, 2) void window_kernel(WindowArgs A) {
                 for (int st = 0; st < NS; ++st)
                     sc[n] = mma32(L::row_frag(sk[buf], n * 32 + (lane & 31), st * 16 + h * 8), qf[st], sc[n]);
             }
-            float mx = m;
+            if (!full) {
+#pragma unroll
+                for (int n = 0; n < NK; ++n)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        if (!A.mask.sees(p, j0 + n * 32 + row_of(r) + 4 * h)) sc[n][r] = -INFINITY;
+            }
+            float mx = sc[0][0];
 #pragma unroll
             for (int n = 0; n < NK; ++n)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    float x = sc[n][r] * A.scale2;
-                    if (!full && !A.mask.sees(p, j0 + n * 32 + row_of(r) + 4 * h)) x = -INFINITY;
-                    sc[n][r] = x;
-                    mx = fmaxf(mx, x);
-                }
+                for (int r = 0; r < 16; ++r) mx = fmaxf(mx, sc[n][r]);
             mx = fmaxf(mx, __shfl_xor(mx, 32));
+            mx = fmaxf(m, mx * scale2);
             const float base = mx == -INFINITY ? 0.f : mx;
             if (__any(mx != m)) {
                 const float alpha = __builtin_amdgcn_exp2f(m - base);
@@ -116,26 +131,34 @@ __global__ __launch_bounds__(256, 2) void window_kernel(WindowArgs A) {
             for (int n = 0; n < NK; ++n)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
-                    sc[n][r] = __builtin_amdgcn_exp2f(sc[n][r] - base);
+                    sc[n][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[n][r], scale2, -base));
                     sum += sc[n][r];
                 }
-            const bool careful = !full && odd;
+            const bool careful = !full && __builtin_amdgcn_readfirstlane(odd);
+            if (!careful) {
 #pragma unroll
-            for (int n = 0; n < NK; ++n)
+                for (int n = 0; n < NK; ++n)
 #pragma unroll
-                for (int k2 = 0; k2 < 2; ++k2) {
-                    const frag<T> pf = next_operand<T>(sc[n], k2);
+                    for (int k2 = 0; k2 < 2; ++k2) {
+                        const frag<T> pf = next_operand<T>(sc[n], k2);
 #pragma unroll
-                    for (int d = 0; d < ND; ++d) {
-                        frag<T> vf = L::col_frag(sv[buf], n * 32 + k2 * 16, d * 32, lane);
-                        if (careful) vf = only_finite<T>(vf);
-                        o[d] = mma32(vf, pf, o[d]);
+                        for (int d = 0; d < ND; ++d)
+                            o[d] = mma32(L::col_frag(sv[buf], n * 32 + k2 * 16, d * 32, lane), pf, o[d]);
                     }
-                }
-            if (careful)
+            } else {
+#pragma unroll
+                for (int n = 0; n < NK; ++n)
+#pragma unroll
+                    for (int k2 = 0; k2 < 2; ++k2) {
+                        const frag<T> pf = next_operand<T>(sc[n], k2);
+#pragma unroll
+                        for (int d = 0; d < ND; ++d)
+                            o[d] = mma32(only_finite<T>(L::col_frag(sv[buf], n * 32 + k2 * 16, d * 32, lane)), pf, o[d]);
+                    }
                 add_not_finite<T, DP>(o, sv[buf], BN, lane, [&](int r) { return A.mask.sees(p, j0 + r); });
+            }
         }
-        if (it + 1 < tiles) stage_store(tile_at(it + 1), buf ^ 1);
+        if (it + 1 < tiles) settle(tile_at(it + 1), buf ^ 1);
         __syncthreads();
     }
     sum += __shfl_xor(sum, 32);

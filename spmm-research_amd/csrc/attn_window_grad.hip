@@ -79,29 +79,34 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void grad_q_kernel(Win
             delta = A.delta[x];
         }
     }
-    Stage<T, DP, GN, 256> ks, vs;
-    auto stage_load = [&](int j0) {
-        auto live = [&](int r) { const int j = j0 + r; return j <= pmax && (j >= lo || j < A.mask.sinks); };
-        ks.load(tid, A.dim, A.k.wide, [&](int r) { return live(r) ? kb + (int64_t)(j0 + r) * A.k.row : nullptr; });
-        vs.load(tid, A.dim, A.v.wide, [&](int r) { return live(r) ? vb + (int64_t)(j0 + r) * A.v.row : nullptr; });
+    using Move = Mover<T, DP, GN, 256>;
+    const bool direct = A.k.wide && A.v.wide;
+    auto key_row = [&](const T *base, const Rows &R, int j) {
+        return j <= pmax && (j >= lo || j < A.mask.sinks) ? base + (int64_t)j * R.row : nullptr;
     };
-    auto stage_store = [&](int j0, int buf) {
-        if (!A.mask.all(pmin, pmax, j0, j0 + GN - 1) && ks.any_not_finite()) odd = 1;
-        ks.store(tid, sk[buf]);
-        vs.store(tid, sv[buf]);
+    auto bring = [&](int j0, int buf, auto how) {
+        how(sk[buf], [&](int r) { return key_row(kb, A.k, j0 + r); });
+        how(sv[buf], [&](int r) { return key_row(vb, A.v, j0 + r); });
+    };
+    auto send = [&](T *tile, auto row) { Move::send(tid, A.dim, tile, row); };
+    auto copy = [&](T *tile, auto row) { Move::copy(tid, A.dim, tile, row); };
+    auto settle = [&](int j0, int buf) {
+        if (direct) Move::arrived();
+        else bring(j0, buf, copy);
+        if (!A.mask.all(pmin, pmax, j0, j0 + GN - 1) && Move::any_not_finite(tid, sk[buf])) odd = 1;
     };
     f32x16 dq[ND];
 #pragma unroll
     for (int d = 0; d < ND; ++d) dq[d] = zero16();
     __syncthreads();
     if (tiles) {
-        stage_load(tile_at(0));
-        stage_store(tile_at(0), 0);
+        if (direct) bring(tile_at(0), 0, send);
+        settle(tile_at(0), 0);
     }
     __syncthreads();
     for (int it = 0; it < tiles; ++it) {
         const int j0 = tile_at(it), buf = it & 1;
-        if (it + 1 < tiles) stage_load(tile_at(it + 1));
+        if (direct && it + 1 < tiles) bring(tile_at(it + 1), buf ^ 1, send);
         if (w0 <= w1 && A.mask.any(w0, w1, j0, j0 + GN - 1)) {
             const bool full = A.mask.all(w0, w1, j0, j0 + GN - 1);
             f32x16 sc = zero16(), dp = zero16();
@@ -115,7 +120,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void grad_q_kernel(Win
                 const float ds = __builtin_amdgcn_exp2f(sc[r] * A.scale2 - lse2) * (dp[r] - delta);
                 sc[r] = full || A.mask.sees(p, j0 + row_of(r) + 4 * h) ? ds : 0.f;
             }
-            const bool careful = !full && odd;      // a seen key that is not finite has made the whole row NaN already
+            const bool careful = !full && __builtin_amdgcn_readfirstlane(odd);      // a seen key that is not finite has made the whole row NaN already
 #pragma unroll
             for (int k2 = 0; k2 < 2; ++k2) {
                 const frag<T> dsf = next_operand<T>(sc, k2);
@@ -127,7 +132,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void grad_q_kernel(Win
                 }
             }
         }
-        if (it + 1 < tiles) stage_store(tile_at(it + 1), buf ^ 1);
+        if (it + 1 < tiles) settle(tile_at(it + 1), buf ^ 1);
         __syncthreads();
     }
     if (!mine) return;
@@ -182,30 +187,33 @@ __global__ __launch_bounds__(256, 1) void grad_kv_kernel(WindowArgs A) {
             vf[st] = load_frag<T>(vr, st * 16 + h * 8, A.dim, A.v.wide);
         }
     }
-    Stage<T, DP, GN, 256> qs, ds;
-    float stat = 0.f;
-    auto stage_load = [&](int it) {
+    using Move = Mover<T, DP, GN, 256>;
+    const bool direct = A.q.wide && A.dout.wide;
+    auto live = [&](int i) { return i >= i0 && i <= i1; };
+    auto bring = [&](int it, int buf, auto how) {
         const int head = kv * group + it / nqt, j0 = (q0t + it % nqt) * GN;
         const T *qb = seq_base<T>(A.q, s, s.q0, packed, head), *db = seq_base<T>(A.dout, s, s.q0, packed, head);
-        auto live = [&](int r) { return j0 + r >= i0 && j0 + r <= i1; };
-        qs.load(tid, A.dim, A.q.wide, [&](int r) { return live(r) ? qb + (int64_t)(j0 + r) * A.q.row : nullptr; });
-        ds.load(tid, A.dim, A.dout.wide, [&](int r) { return live(r) ? db + (int64_t)(j0 + r) * A.dout.row : nullptr; });
-        if (tid < 2 * GN) {
-            const int r = tid % GN;
-            const int64_t x = ((packed ? s.q0 : s.b * A.q_len) + j0 + r) * A.heads + head;
-            if (tid < GN) {
-                stat = INFINITY;                     // no row, or one that sees nothing: P = exp2(x - inf) = 0
-                if (live(r) && A.lse[x] != -INFINITY) stat = A.lse[x] * LOG2E;
-            } else {
-                stat = live(r) ? A.delta[x] : 0.f;
-            }
-        }
+        how(sq[buf], [&](int r) { return live(j0 + r) ? qb + (int64_t)(j0 + r) * A.q.row : nullptr; });
+        how(sd[buf], [&](int r) { return live(j0 + r) ? db + (int64_t)(j0 + r) * A.dout.row : nullptr; });
     };
-    auto stage_store = [&](int it, int buf) {
-        const int j0 = (q0t + it % nqt) * GN + shift;
-        if (!A.mask.all(j0, j0 + GN - 1, n0, n1) && (qs.any_not_finite() || ds.any_not_finite())) odd = 1;
-        qs.store(tid, sq[buf]);
-        ds.store(tid, sd[buf]);
+    float stat = 0.f;                                // lse or delta of one of the tile's rows, on its way to LDS
+    auto load_stat = [&](int it) {
+        if (tid >= 2 * GN) return;
+        const int head = kv * group + it / nqt, i = (q0t + it % nqt) * GN + tid % GN;
+        const int64_t x = ((packed ? s.q0 : s.b * A.q_len) + i) * A.heads + head;
+        stat = tid < GN ? INFINITY : 0.f;            // no row, or one that sees nothing: P = exp2(x - inf) = 0
+        if (!live(i)) return;
+        if (tid >= GN) stat = A.delta[x];
+        else if (A.lse[x] != -INFINITY) stat = A.lse[x] * LOG2E;
+    };
+    auto send = [&](T *tile, auto row) { Move::send(tid, A.dim, tile, row); };
+    auto copy = [&](T *tile, auto row) { Move::copy(tid, A.dim, tile, row); };
+    auto settle = [&](int it, int buf) {
+        const int p0 = (q0t + it % nqt) * GN + shift;
+        if (direct) Move::arrived();
+        else bring(it, buf, copy);
+        if (!A.mask.all(p0, p0 + GN - 1, n0, n1) &&
+            (Move::any_not_finite(tid, sq[buf]) || Move::any_not_finite(tid, sd[buf]))) odd = 1;
         if (tid < GN) slse[buf][tid] = stat;
         else if (tid < 2 * GN) sdelta[buf][tid - GN] = stat;
     };
@@ -214,13 +222,17 @@ __global__ __launch_bounds__(256, 1) void grad_kv_kernel(WindowArgs A) {
     for (int d = 0; d < ND; ++d) dk[d] = dv[d] = zero16();
     __syncthreads();
     if (tiles) {
-        stage_load(0);
-        stage_store(0, 0);
+        load_stat(0);
+        if (direct) bring(0, 0, send);
+        settle(0, 0);
     }
     __syncthreads();
     for (int it = 0; it < tiles; ++it) {
         const int j0 = (q0t + it % nqt) * GN, p0 = j0 + shift, buf = it & 1;
-        if (it + 1 < tiles) stage_load(it + 1);
+        if (it + 1 < tiles) {
+            load_stat(it + 1);
+            if (direct) bring(it + 1, buf ^ 1, send);
+        }
         if (c0 <= c1 && A.mask.any(p0, p0 + GN - 1, c0, c1)) {
             const bool full = A.mask.all(p0, p0 + GN - 1, c0, c1);
             f32x16 sc = zero16(), dp = zero16();
@@ -241,7 +253,7 @@ __global__ __launch_bounds__(256, 1) void grad_kv_kernel(WindowArgs A) {
                     sc[r] = seen ? pr : 0.f;
                 }
             }
-            const bool careful = !full && odd;
+            const bool careful = !full && __builtin_amdgcn_readfirstlane(odd);
 #pragma unroll
             for (int k2 = 0; k2 < 2; ++k2) {
                 const frag<T> pf = next_operand<T>(sc, k2), dsf = next_operand<T>(dp, k2);
@@ -259,7 +271,7 @@ __global__ __launch_bounds__(256, 1) void grad_kv_kernel(WindowArgs A) {
             if (careful)
                 add_not_finite<T, DP>(dv, sd[buf], GN, lane, [&](int r) { return j0 + r <= i1 && A.mask.sees(p0 + r, key); });
         }
-        if (it + 1 < tiles) stage_store(it + 1, buf ^ 1);
+        if (it + 1 < tiles) settle(it + 1, buf ^ 1);
         __syncthreads();
     }
     if (!mine) return;

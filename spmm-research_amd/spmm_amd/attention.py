@@ -63,29 +63,30 @@ def _check(where: str, st: int) -> None:
         raise SpmmHipError(where, st, (lib.spmm_attn_last_error_detail() or b"").decode())
 
 
-def _tensor(name: str, t, like=None, shape=None, dtype=None, contiguous=False):
-    """t is a tensor on a HIP device, of like's device and dtype, of the given shape, its rows contiguous."""
+def _tensor(name: str, t, dtype=None, device: int | None = None, shape=None, contiguous: bool = False) -> tuple:
+    """t is a tensor on a HIP device (the given one), of the given dtype and shape, its innermost dimension (or all of it)
+    contiguous: its strides."""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch tensor")
-    if t.device.type != "cuda":
+    if not t.is_cuda:
         raise ValueError(f"{name} is on {t.device}: there is no CPU path")
-    want = dtype if dtype is not None else like.dtype if like is not None else None
-    if want is not None and t.dtype != want:
-        raise TypeError(f"{name} is {t.dtype}, expected {want}")
-    if like is not None and t.device != like.device:
-        raise ValueError(f"{name} is on {t.device}, expected {like.device}")
-    if shape is not None and tuple(t.shape) != tuple(shape):
+    if dtype is not None and t.dtype is not dtype:
+        raise TypeError(f"{name} is {t.dtype}, expected {dtype}")
+    if device is not None and t.get_device() != device:
+        raise ValueError(f"{name} is on {t.device}, expected HIP device {device}")
+    if shape is not None and t.shape != shape:
         raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
-    if contiguous and not t.is_contiguous():
-        raise ValueError(f"{name} must be contiguous")
-    if not contiguous and t.ndim and t.shape[-1] > 1 and t.stride(-1) != 1 and t.numel():
-        raise ValueError(f"the innermost dimension of {name} must be contiguous")
-    return t
-
-
-def _rows(t, packed: bool = False) -> _Rows:
-    """[batch, rows, heads, d], or [rows, heads, d] with offsets."""
     s = t.stride()
+    if contiguous:
+        if not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous")
+    elif s and s[-1] != 1 and t.shape[-1] > 1 and t.numel():
+        raise ValueError(f"the innermost dimension of {name} must be contiguous")
+    return s
+
+
+def _rows(t, s: tuple, packed: bool = False) -> _Rows:
+    """[batch, rows, heads, d], or [rows, heads, d] with offsets, of strides s."""
     return _Rows(t.data_ptr(), 0, s[0], s[1]) if packed else _Rows(t.data_ptr(), s[0], s[1], s[2])
 
 
@@ -97,50 +98,55 @@ def _int(name: str, x, lo: int, hi: int = 2 ** 31 - 1) -> int:
     return x
 
 
-def _place(t, stream):
-    """(stream handle, context in which allocations belong to that stream)."""
+def _place(device: int, stream):
+    """(stream handle, context in which allocations belong to that stream, None where they do already)."""
     if stream is None:
-        return torch.cuda.current_stream(t.device).cuda_stream, contextlib.nullcontext()
+        return torch._C._cuda_getCurrentRawStream(device), None
     if isinstance(stream, bool) or not isinstance(stream, int):
         raise TypeError("stream must be an integer hipStream_t")
-    return stream, torch.cuda.stream(torch.cuda.ExternalStream(stream, device=t.device))
+    return stream, torch.cuda.stream(torch.cuda.ExternalStream(stream, device=device))
 
 
-def _desc(q, kv_heads: int, window, sinks, scale, batch: int, q_len: int, k_len: int, zero_rest: bool = False) -> _Desc:
-    heads, dim = q.shape[-2], q.shape[-1]
-    if q.dtype not in _DTYPES:
+_HERE = contextlib.nullcontext()
+
+
+def _desc(q, device: int, kv_heads: int, window, sinks, scale, batch: int, q_len: int, k_len: int, zero_rest: bool = False) -> _Desc:
+    heads, dim = q.shape[-2:]
+    dtype = _DTYPES.get(q.dtype)
+    if dtype is None:
         raise TypeError(f"element type {q.dtype}: float32, float16 or bfloat16")
     if not 1 <= dim <= MAX_DIM:
         raise ValueError(f"head width {dim} is not in 1 .. {MAX_DIM}")
     if kv_heads < 1 or heads < 1 or heads % kv_heads:
         raise ValueError(f"{heads} heads are not a multiple of {kv_heads} key heads")
-    return _Desc(q.device.index, _DTYPES[q.dtype], heads, kv_heads, dim, _int("window", window, 0),
-                 _int("sinks", sinks, 0), dim ** -0.5 if scale is None else float(scale), batch, q_len, k_len,
-                 int(zero_rest), 0)
+    return _Desc(device, dtype, heads, kv_heads, dim, _int("window", window, 0), _int("sinks", sinks, 0),
+                 dim ** -0.5 if scale is None else scale, batch, q_len, k_len, zero_rest, 0)
 
 
 def _window_operands(q, k, v, window, sinks, scale, cu_q, cu_k, zero_rest):
+    """(packed, description, addresses of the offsets, rows of q, k, v, device, dtype)"""
     packed = cu_q is not None
     if not packed and cu_k is not None:
         raise ValueError("cu_k without cu_q")
+    qs = _tensor("q", q)
+    dev, dt = q.get_device(), q.dtype
+    ks, vs = _tensor("k", k, dt, dev), _tensor("v", v, dt, dev)
     nd = 3 if packed else 4
-    _tensor("q", q)
-    _tensor("k", k, q)
-    _tensor("v", v, q)
-    if q.ndim != nd or k.ndim != nd or v.ndim != nd:
+    if len(qs) != nd or len(ks) != nd or len(vs) != nd:
         raise ValueError(f"q, k and v need {nd} dimensions: " + ("[rows, heads, d]" if packed else "[batch, rows, heads, d]"))
-    if k.shape != v.shape or k.shape[-1] != q.shape[-1] or (not packed and k.shape[0] != q.shape[0]):
-        raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not fit")
-    batch = q.shape[0]
+    qd, kd = q.shape, k.shape
+    if kd != v.shape or kd[-1] != qd[-1] or (not packed and kd[0] != qd[0]):
+        raise ValueError(f"q {tuple(qd)}, k {tuple(kd)} and v {tuple(v.shape)} do not fit")
+    batch, pq, pk = qd[0], None, None
     if packed:
         cu_k = cu_q if cu_k is None else cu_k
-        _tensor("cu_q", cu_q, q, dtype=torch.int32, contiguous=True)
-        _tensor("cu_k", cu_k, q, dtype=torch.int32, contiguous=True)
+        _tensor("cu_q", cu_q, torch.int32, dev, None, True)
+        _tensor("cu_k", cu_k, torch.int32, dev, None, True)
         if cu_q.ndim != 1 or cu_q.shape != cu_k.shape or len(cu_q) < 1:
             raise ValueError("cu_q and cu_k must be vectors of the number of sequences + 1")
-        batch = len(cu_q) - 1
-    d = _desc(q, k.shape[-2], window, sinks, scale, batch, q.shape[-3], k.shape[-3], zero_rest and packed)
-    return packed, d, cu_q.data_ptr() if packed else None, cu_k.data_ptr() if packed else None
+        batch, pq, pk = len(cu_q) - 1, cu_q.data_ptr(), cu_k.data_ptr()
+    d = _desc(q, dev, kd[-2], window, sinks, scale, batch, qd[-3], kd[-3], zero_rest and packed)
+    return packed, d, pq, pk, _rows(q, qs, packed), _rows(k, ks, packed), _rows(v, vs, packed), dev, dt
 
 
 def window_attention(q, k, v, window: int = 0, sinks: int = 0, scale: float | None = None, cu_q=None, cu_k=None,
@@ -152,21 +158,21 @@ def window_attention(q, k, v, window: int = 0, sinks: int = 0, scale: float | No
     ``scale`` defaults to d ** -0.5.  out is like q, lse float32 with q's shape less its last dimension (the log of the sum
     of the exponentials, -inf where a query sees nothing).  With offsets, rows behind the last sequence are set to 0
     (lse -inf) in an out that the call allocates and left as they are, in lse too, if ``out`` is given."""
-    packed, d, pq, pk = _window_operands(q, k, v, window, sinks, scale, cu_q, cu_k, out is None)
-    st, where = _place(q, stream)
-    with where:
+    packed, d, pq, pk, qr, kr, vr, dev, dt = _window_operands(q, k, v, window, sinks, scale, cu_q, cu_k, out is None)
+    st, where = _place(dev, stream)
+    with where or _HERE:
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            out = torch.empty(q.shape, dtype=dt, device=q.device)
+            os = out.stride()
         else:
-            _tensor("out", out, q, q.shape)
+            os = _tensor("out", out, dt, dev, q.shape)
         if lse is None:
             lse = torch.empty(q.shape[:-1], dtype=torch.float32, device=q.device)
         else:
-            _tensor("lse", lse, q, q.shape[:-1], torch.float32, True)
+            _tensor("lse", lse, torch.float32, dev, q.shape[:-1], True)
         if packed and d.batch == 0 and d.zero_rest:
             return out.zero_(), lse.fill_(float("-inf"))
-    _check("window_attention", lib.spmm_attn_window(d, _rows(q, packed), _rows(k, packed), _rows(v, packed), pq, pk,
-                                                    _rows(out, packed), lse.data_ptr(), st))
+    _check("window_attention", lib.spmm_attn_window(d, qr, kr, vr, pq, pk, _rows(out, os, packed), lse.data_ptr(), st))
     return out, lse
 
 
@@ -175,39 +181,45 @@ def window_attention_backward(dout, q, k, v, out, lse, window: int = 0, sinks: i
     """Gradients (dq, dk, dv) of ``window_attention`` for the gradient ``dout`` of its out; out, lse: what it returned,
     the other arguments as they were.  With offsets, rows behind the last sequence are set to 0 if the call allocates
     all three, and left as they are if any is given."""
-    packed, d, pq, pk = _window_operands(q, k, v, window, sinks, scale, cu_q, cu_k, dq is None and dk is None and dv is None)
-    _tensor("dout", dout, q, q.shape)
-    _tensor("out", out, q, q.shape)
-    _tensor("lse", lse, q, q.shape[:-1], torch.float32, True)
-    st, where = _place(q, stream)
+    packed, d, pq, pk, qr, kr, vr, dev, dt = _window_operands(q, k, v, window, sinks, scale, cu_q, cu_k,
+                                                              dq is None and dk is None and dv is None)
+    dr = _rows(dout, _tensor("dout", dout, dt, dev, q.shape), packed)
+    outr = _rows(out, _tensor("out", out, dt, dev, q.shape), packed)
+    _tensor("lse", lse, torch.float32, dev, q.shape[:-1], True)
+    st, where = _place(dev, stream)
     need = C.c_size_t()
-    _check("window_attention_backward", lib.spmm_attn_window_work(d, int(packed), C.byref(need)))
-    with where:
-        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) if g is None else _tensor(n, g, q, t.shape)
-                      for n, g, t in (("dq", dq, q), ("dk", dk, k), ("dv", dv, v)))
+    _check("window_attention_backward", lib.spmm_attn_window_work(d, packed, need))
+    with where or _HERE:
+        res, rows = [], []
+        for name, g, t in (("dq", dq, q), ("dk", dk, k), ("dv", dv, v)):
+            if g is None:
+                g = torch.empty(t.shape, dtype=dt, device=t.device)
+                s = g.stride()
+            else:
+                s = _tensor(name, g, dt, dev, t.shape)
+            res.append(g)
+            rows.append(_rows(g, s, packed))
         work = torch.empty(need.value, dtype=torch.uint8, device=q.device)
         if packed and d.batch == 0 and d.zero_rest:
-            return dq.zero_(), dk.zero_(), dv.zero_()
-    _check("window_attention_backward", lib.spmm_attn_window_grad(
-        d, _rows(dout, packed), _rows(q, packed), _rows(k, packed), _rows(v, packed), _rows(out, packed), lse.data_ptr(),
-        pq, pk, _rows(dq, packed), _rows(dk, packed), _rows(dv, packed), work.data_ptr(), need.value, st))
-    return dq, dk, dv
+            return tuple(g.zero_() for g in res)
+    _check("window_attention_backward", lib.spmm_attn_window_grad(d, dr, qr, kr, vr, outr, lse.data_ptr(), pq, pk, *rows,
+                                                                  work.data_ptr(), need.value, st))
+    return tuple(res)
 
 
-def _pages(k_pages, v_pages, page_table, lengths, like, batch: int) -> _Pages:
-    _tensor("k_pages", k_pages, like)
-    _tensor("v_pages", v_pages, like)
-    if k_pages.ndim != 4 or k_pages.shape != v_pages.shape or k_pages.shape[3] != like.shape[-1]:
-        raise ValueError(f"pages {tuple(k_pages.shape)} and {tuple(v_pages.shape)}: [pages, rows, key heads, d] expected")
-    if k_pages.shape[1] < 1:
+def _pages(k_pages, v_pages, page_table, lengths, dim: int, dt, dev: int, batch: int) -> _Pages:
+    ks, vs = _tensor("k_pages", k_pages, dt, dev), _tensor("v_pages", v_pages, dt, dev)
+    shape = k_pages.shape
+    if len(ks) != 4 or shape != v_pages.shape or shape[3] != dim:
+        raise ValueError(f"pages {tuple(shape)} and {tuple(v_pages.shape)}: [pages, rows, key heads, {dim}] expected")
+    if shape[1] < 1:
         raise ValueError("pages without rows")
-    _tensor("page_table", page_table, like, dtype=torch.int32)
-    if page_table.ndim != 2 or page_table.shape[0] != batch:
+    ts = _tensor("page_table", page_table, torch.int32, dev)
+    if len(ts) != 2 or page_table.shape[0] != batch:
         raise ValueError(f"page_table {tuple(page_table.shape)}: one row for each of {batch} sequences expected")
-    _tensor("lengths", lengths, like, (batch,), torch.int32, True)
-    ks, vs = k_pages.stride(), v_pages.stride()
-    return _Pages(k_pages.data_ptr(), v_pages.data_ptr(), k_pages.shape[0], k_pages.shape[1], ks[0], ks[1], ks[2], vs[0],
-                  vs[1], vs[2], page_table.data_ptr(), page_table.shape[1], page_table.stride(0), lengths.data_ptr())
+    _tensor("lengths", lengths, torch.int32, dev, (batch,), True)
+    return _Pages(k_pages.data_ptr(), v_pages.data_ptr(), shape[0], shape[1], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2],
+                  page_table.data_ptr(), page_table.shape[1], ts[0], lengths.data_ptr())
 
 
 def paged_attention(q, k_pages, v_pages, page_table, lengths, window: int = 0, sinks: int = 0,
@@ -221,24 +233,28 @@ def paged_attention(q, k_pages, v_pages, page_table, lengths, window: int = 0, s
     lengths (by default what the table can hold); a tight one gives the better split of the work.  A sequence whose
     visible positions need a page that is not there, or whose length is negative, above max_length or above what the table
     can hold, gets NaN."""
-    _tensor("q", q)
-    if q.ndim != 3:
+    qs = _tensor("q", q)
+    if len(qs) != 3:
         raise ValueError(f"q {tuple(q.shape)}: [batch, heads, d] expected")
-    pages = _pages(k_pages, v_pages, page_table, lengths, q, q.shape[0])
-    d = _desc(q, k_pages.shape[2], window, sinks, scale, q.shape[0], 1, 0)
-    room = min(page_table.shape[1] * k_pages.shape[1], 2 ** 30 - 1)
+    dev, dt, batch = q.get_device(), q.dtype, q.shape[0]
+    pages = _pages(k_pages, v_pages, page_table, lengths, q.shape[2], dt, dev, batch)
+    d = _desc(q, dev, k_pages.shape[2], window, sinks, scale, batch, 1, 0)
+    room = min(pages.table_cols * pages.page_rows, 2 ** 30 - 1)
     longest = room if max_length is None else min(_int("max_length", max_length, 0), room)
-    st, where = _place(q, stream)
+    st, where = _place(dev, stream)
     need = C.c_size_t()
-    _check("paged_attention", lib.spmm_attn_paged_work(d, longest, C.byref(need)))
-    with where:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None else _tensor("out", out, q, q.shape)
+    _check("paged_attention", lib.spmm_attn_paged_work(d, longest, need))
+    with where or _HERE:
+        if out is None:
+            out = torch.empty(q.shape, dtype=dt, device=q.device)
+            os = out.stride()
+        else:
+            os = _tensor("out", out, dt, dev, q.shape)
         if lse is None:
             lse = torch.empty(q.shape[:-1], dtype=torch.float32, device=q.device)
         else:
-            _tensor("lse", lse, q, q.shape[:-1], torch.float32, True)
+            _tensor("lse", lse, torch.float32, dev, q.shape[:-1], True)
         work = torch.empty(need.value, dtype=torch.uint8, device=q.device) if need.value else None
-    qs, os = q.stride(), out.stride()
     _check("paged_attention", lib.spmm_attn_paged(
         d, _Rows(q.data_ptr(), qs[0], 0, qs[1]), pages, longest, _Rows(out.data_ptr(), os[0], 0, os[1]), lse.data_ptr(),
         work.data_ptr() if work is not None else None, need.value, st))
@@ -250,19 +266,20 @@ def cache_append(k, v, k_pages, v_pages, page_table, lengths, cu=None, stream: i
     ``lengths[b]``.  k and v [batch, key heads, d], one token a sequence (none for a sequence of length 0), or, with
     int32 offsets ``cu`` [batch + 1] on the device, [rows, key heads, d].  Rows whose page is not there are dropped.  A
     page that is written must belong to one sequence only."""
-    _tensor("k", k)
-    _tensor("v", v, k, k.shape)
-    if k.ndim != 3:
+    ks = _tensor("k", k)
+    dev, dt = k.get_device(), k.dtype
+    vs = _tensor("v", v, dt, dev, k.shape)
+    if len(ks) != 3:
         raise ValueError(f"k {tuple(k.shape)}: [rows, key heads, d] expected")
+    rows, heads, dim = k.shape
+    batch, pc = rows, None
     if cu is not None:
-        _tensor("cu", cu, k, dtype=torch.int32, contiguous=True)
+        _tensor("cu", cu, torch.int32, dev, None, True)
         if cu.ndim != 1 or len(cu) < 1:
             raise ValueError("cu must be a vector of the number of sequences + 1")
-    batch = k.shape[0] if cu is None else len(cu) - 1
-    pages = _pages(k_pages, v_pages, page_table, lengths, k, batch)
-    if k_pages.shape[2] != k.shape[1]:
-        raise ValueError(f"{k.shape[1]} key heads, the pages have {k_pages.shape[2]}")
-    d = _desc(k, k.shape[1], 0, 0, 1.0, batch, k.shape[0], 0)
-    st, _ = _place(k, stream)
-    _check("cache_append", lib.spmm_attn_append(d, _rows(k, True), _rows(v, True), cu.data_ptr() if cu is not None else None,
-                                                pages, st))
+        batch, pc = len(cu) - 1, cu.data_ptr()
+    pages = _pages(k_pages, v_pages, page_table, lengths, dim, dt, dev, batch)
+    if k_pages.shape[2] != heads:
+        raise ValueError(f"{heads} key heads, the pages have {k_pages.shape[2]}")
+    _check("cache_append", lib.spmm_attn_append(_desc(k, dev, heads, 0, 0, 1.0, batch, rows, 0), _rows(k, ks, True),
+                                                _rows(v, vs, True), pc, pages, _place(dev, stream)[0]))

@@ -13,7 +13,7 @@ import ctypes as C
 import torch
 
 from . import SpmmHipError, _open
-from .attention import F16, BF16, F32, _int, _place, _tensor
+from .attention import F16, BF16, F32, _HERE, _int, _place, _tensor
 
 _DTYPES = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
 
@@ -50,13 +50,12 @@ class Q4Format:
     format_name = "HIP_Q4_MI355X"
 
     def __init__(self, packed, scales, zeros=None, cols: int | None = None, group: int = 128, stream: int | None = None):
-        _tensor("packed", packed, dtype=torch.uint8)
-        _tensor("scales", scales)
-        if packed.device != scales.device:
-            raise ValueError(f"scales are on {scales.device}, expected {packed.device}")
+        ps = _tensor("packed", packed, torch.uint8)
+        dev = packed.get_device()
+        ss = _tensor("scales", scales, None, dev)
         if scales.dtype not in _DTYPES:
             raise TypeError(f"scales are {scales.dtype}: float32, float16 or bfloat16")
-        if packed.ndim != 2 or scales.ndim != 2:
+        if len(ps) != 2 or len(ss) != 2:
             raise ValueError("packed and scales must have two dimensions")
         self.rows = packed.shape[0]
         self.cols = 2 * packed.shape[1] if cols is None else _int("cols", cols, 0)
@@ -65,43 +64,38 @@ class Q4Format:
             raise ValueError(f"packed has {packed.shape[1]} bytes a row, {self.cols} columns need {(self.cols + 1) // 2}")
         shape = (self.rows, -(-self.cols // self.group))
         _tensor("scales", scales, shape=shape)
-        if zeros is not None:
-            _tensor("zeros", zeros, shape=shape, dtype=torch.uint8)
-            if zeros.device != packed.device:
-                raise ValueError(f"zeros are on {zeros.device}, expected {packed.device}")
+        zs = _tensor("zeros", zeros, torch.uint8, dev, shape) if zeros is not None else (0, 0)
         self.dtype, self.device = scales.dtype, packed.device
-        self._d = _Desc(packed.device.index, _DTYPES[scales.dtype], self.rows, self.cols, self.group, int(zeros is not None))
+        self._dev = dev
+        self._d = _Desc(dev, _DTYPES[scales.dtype], self.rows, self.cols, self.group, int(zeros is not None))
         need = C.c_size_t()
-        _check("Q4Format", lib.spmm_q4_layout_bytes(self._d, C.byref(need)))
-        st, where = _place(packed, stream)
-        with where:
+        _check("Q4Format", lib.spmm_q4_layout_bytes(self._d, need))
+        st, where = _place(dev, stream)
+        with where or _HERE:
             self._layout = torch.empty(need.value, dtype=torch.uint8, device=packed.device)
         self.mem_footprint = float(need.value)
-        _check("Q4Format", lib.spmm_q4_layout(self._d, packed.data_ptr(), packed.stride(0), scales.data_ptr(),
-                                              scales.stride(0), zeros.data_ptr() if zeros is not None else None,
-                                              zeros.stride(0) if zeros is not None else 0, self._layout.data_ptr(),
-                                              need.value, st))
+        _check("Q4Format", lib.spmm_q4_layout(self._d, packed.data_ptr(), ps[0], scales.data_ptr(), ss[0],
+                                              zeros.data_ptr() if zeros is not None else None, zs[0],
+                                              self._layout.data_ptr(), need.value, st))
 
     def matvec(self, x, out=None, stream: int | None = None):
         """x W^T: x [cols] or [tokens, cols] (rows any distance apart) -> [rows] or [tokens, rows].  Made for a few
         vectors: every 16 of them (5 in float32) read the weights once more.  A call on another stream than the one the
         format was made on has to come after it."""
-        _tensor("x", x, dtype=self.dtype)
-        if x.device != self.device:
-            raise ValueError(f"x is on {x.device}, expected {self.device}")
-        if x.ndim not in (1, 2) or x.shape[-1] != self.cols:
+        xs = _tensor("x", x, self.dtype, self._dev)
+        nd = len(xs)
+        if nd not in (1, 2) or x.shape[-1] != self.cols:
             raise ValueError(f"x {tuple(x.shape)}: [{self.cols}] or [tokens, {self.cols}] expected")
-        tokens = 1 if x.ndim == 1 else x.shape[0]
-        shape = x.shape[:-1] + (self.rows,)
-        st, where = _place(x, stream)
-        if out is not None:
-            _tensor("out", out, x, shape)
-        else:
-            with where:
-                out = torch.empty(shape, dtype=x.dtype, device=x.device)
-        if self.cols == 0:
-            with where:
+        shape = (self.rows,) if nd == 1 else (x.shape[0], self.rows)
+        st, where = _place(self._dev, stream)
+        with where or _HERE:
+            if out is None:
+                out = torch.empty(shape, dtype=self.dtype, device=self.device)
+                os = out.stride()
+            else:
+                os = _tensor("out", out, self.dtype, self._dev, shape)
+            if self.cols == 0:
                 return out.zero_()
-        _check("matvec", lib.spmm_q4_matvec(self._d, self._layout.data_ptr(), x.data_ptr(), x.stride(0) if x.ndim == 2 else 0,
-                                            tokens, out.data_ptr(), out.stride(0) if x.ndim == 2 else self.rows, st))
+        _check("matvec", lib.spmm_q4_matvec(self._d, self._layout.data_ptr(), x.data_ptr(), xs[0] if nd == 2 else 0,
+                                            x.shape[0] if nd == 2 else 1, out.data_ptr(), os[0] if nd == 2 else self.rows, st))
         return out
