@@ -27,7 +27,7 @@ struct PagedArgs {
     const int32_t *table, *lengths;
     bool k_wide, v_wide;
     int64_t batch, limit;                    // limit: longest sequence allowed
-    int heads, kv_heads, dim, window, sinks, splits;
+    int heads, kv_heads, dim, window, sinks, splits, page_shift;      // page_shift: of a power of two, else -1
     float scale2;
     float *lse, *part;                       // part: [batch][heads][splits][dim + 2]: max, sum, weighted values
 };
@@ -46,30 +46,23 @@ __device__ __forceinline__ Span span_of(int len, int window, int sinks) {
     return s;
 }
 
-// V elements a lane owns: VE = dim rounded up to 16 VE; value column of lane n, element j is n * VE + j.
-template <typename T, int VE> struct VRow {
-    float x[VE];
-    __device__ __forceinline__ void load(const T *row, int n, int dim, bool wide) {
-        const int e = n * VE;
-        if (!row || e >= dim) {
+__device__ __align__(16) const float zero_row[SPMM_ATTN_MAX_DIM] = {};
+
+// E elements of a row from element e on, zero beyond dim; `row` is zero_row where there is none.
+template <typename T, int E> struct Piece {
+    typedef T vec __attribute__((ext_vector_type(E)));
+    static __device__ __forceinline__ vec load(const T *row, int e, int dim, bool wide) {
+        if (wide) return *reinterpret_cast<const vec *>(e < dim ? row + e : (const T *)zero_row);
+        vec v;
 #pragma unroll
-            for (int j = 0; j < VE; ++j) x[j] = 0.f;
-            return;
-        }
-        if (wide && e + VE <= dim) {
-            typedef T vec __attribute__((ext_vector_type(VE)));
-            const vec w = *reinterpret_cast<const vec *>(row + e);
-#pragma unroll
-            for (int j = 0; j < VE; ++j) x[j] = (float)w[j];
-        } else {
-#pragma unroll
-            for (int j = 0; j < VE; ++j) x[j] = e + j < dim ? (float)row[e + j] : 0.f;
-        }
+        for (int j = 0; j < E; ++j) v[j] = e + j < dim ? row[e + j] : (T)0.f;
+        return v;
     }
 };
 
 template <typename T, int DP>
-__global__ __launch_bounds__(PW * 64) void paged_kernel(PagedArgs A) {
+__global__ __launch_bounds__(PW * 64, sizeof(T) == 2 ? 4 : 2) void paged_kernel(PagedArgs A) {
+    // a lane's columns of the values: VE from VE (lane % 16) on
     constexpr int NS = DP / 32, VE = DP / 16;
     const int group = A.heads / A.kv_heads, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, h4 = lane >> 4;
     const int hb = (group + 15) / 16;                       // blocks of 16 query heads of a group
@@ -95,34 +88,46 @@ __global__ __launch_bounds__(PW * 64) void paged_kernel(PagedArgs A) {
     }
     const T *kb = (const T *)A.k + kv * A.k_head, *vb = (const T *)A.v + kv * A.v_head;
     const int32_t *table = A.table + b * A.table_stride;
+    auto seen = [&](int j) { return j < len && (A.window == 0 || len - 1 - j < A.window || j < A.sinks); };
+    // page and row of this lane's key n of tile t; the page is -1 if the key is not seen
+    auto locate = [&](int t, int &slot) -> int {
+        const int j = t < t1 ? sp.at(t) + n : len;
+        uint32_t c;
+        if (A.page_shift >= 0) {
+            c = (uint32_t)j >> A.page_shift;
+            slot = j - (int)(c << A.page_shift);
+        } else {
+            c = (uint32_t)j / (uint32_t)A.page_rows;
+            slot = j - (int)(c * (uint32_t)A.page_rows);
+        }
+        if (!seen(j)) return -1;
+        const int pg = table[c];
+        return pg < 0 || pg >= A.pages ? -2 : pg;
+    };
 
     f32x4 o[VE];
 #pragma unroll
     for (int j = 0; j < VE; ++j) o[j] = f32x4{0.f, 0.f, 0.f, 0.f};
     float m = -INFINITY, sum = 0.f;
+    int slot_next, page_next = locate(t0 + wave, slot_next);
     for (int t = t0 + wave; t < t1; t += PW) {
-        const int j0 = sp.at(t);
-        auto seen = [&](int j) { return j < len && (A.window == 0 || len - 1 - j < A.window || j < A.sinks); };
-        // row of position j in the pages, -1 if it is not seen
-        auto find = [&](int j) -> int64_t {
-            if (!seen(j)) return -1;
-            const int64_t pg = table[j / A.page_rows];
-            if (pg < 0 || pg >= A.pages) { bad = true; return -1; }
-            return pg;
-        };
-        const int jk = j0 + n;
-        const int64_t pk = find(jk);
-        const T *kr = pk < 0 ? nullptr : kb + pk * A.k_page + (jk % A.page_rows) * A.k_row;
-        f32x4 sc = {0.f, 0.f, 0.f, 0.f};
+        const int j0 = sp.at(t), page = page_next, slot = slot_next;
+        page_next = locate(t + PW, slot_next);
+        bad |= page == -2;
+        const int64_t voff = page < 0 ? -1 : (int64_t)page * A.v_page + slot * A.v_row;
+        const T *kr = page < 0 ? (const T *)zero_row : kb + (int64_t)page * A.k_page + slot * A.k_row;
+        frag<T> kf[NS];
 #pragma unroll
-        for (int s = 0; s < NS; ++s) sc = mma16(load_frag<T>(kr, s * 32 + h4 * 8, A.dim, A.k_wide), qf[s], sc);
-        VRow<T, VE> vr[4];
+        for (int s = 0; s < NS; ++s) kf[s] = Piece<T, 8>::load(kr, s * 32 + h4 * 8, A.dim, A.k_wide);
+        typename Piece<T, VE>::vec vr[4];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            const int j = j0 + 4 * h4 + r;
-            const int64_t pv = find(j);
-            vr[r].load(pv < 0 ? nullptr : vb + pv * A.v_page + (j % A.page_rows) * A.v_row, n, A.dim, A.v_wide);
+            const int64_t off = __shfl(voff, 4 * h4 + r);
+            vr[r] = Piece<T, VE>::load(off < 0 ? (const T *)zero_row : vb + off, n * VE, A.dim, A.v_wide);
         }
+        f32x4 sc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = 0; s < NS; ++s) sc = mma16(kf[s], qf[s], sc);
         float mx = m;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
@@ -150,7 +155,8 @@ __global__ __launch_bounds__(PW * 64) void paged_kernel(PagedArgs A) {
 #pragma unroll
         for (int r = 0; r < 4; ++r)
 #pragma unroll
-            for (int j = 0; j < VE; ++j) o[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(sc[r], vr[r].x[j], o[j], 0, 0, 0);
+            for (int j = 0; j < VE; ++j)
+                o[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(sc[r], (float)vr[r][j], o[j], 0, 0, 0);
     }
     sum += __shfl_xor(sum, 16);
     sum += __shfl_xor(sum, 32);
@@ -197,26 +203,40 @@ __global__ __launch_bounds__(PW * 64) void paged_kernel(PagedArgs A) {
     }
 }
 
-// One wave a (sequence, head): its parts joined in order.
+// One wave a (sequence, head): its parts joined in an order that is fixed by their number.
 template <typename T> __global__ __launch_bounds__(64) void paged_join_kernel(PagedArgs A) {
     const int64_t x = blockIdx.x, b = x / A.heads;
-    const int hd = (int)(x % A.heads), lane = threadIdx.x;
-    const float *p = A.part + x * A.splits * (A.dim + 2);
+    const int hd = (int)(x % A.heads), lane = threadIdx.x, w = A.dim + 2;
+    const float *p = A.part + x * A.splits * w;
     float mx = -INFINITY;
-    for (int s = 0; s < A.splits; ++s) mx = fmaxf(mx, p[s * (A.dim + 2)]);
+    for (int s = lane; s < A.splits; s += WAVE) mx = fmaxf(mx, p[(int64_t)s * w]);
+#pragma unroll
+    for (int d = 32; d; d /= 2) mx = fmaxf(mx, __shfl_xor(mx, d));
     const float base = mx == -INFINITY ? 0.f : mx;
     float tot = 0.f, a0 = 0.f, a1 = 0.f;
-    for (int s = 0; s < A.splits; ++s) {
-        const float *ps = p + s * (A.dim + 2);
-        const float f = __builtin_amdgcn_exp2f(ps[0] - base);
-        tot += f * ps[1];
-        if (lane < A.dim) a0 += f * ps[2 + lane];
-        if (lane + 64 < A.dim) a1 += f * ps[2 + lane + 64];
+    const int e0 = min(lane, A.dim - 1), e1 = min(lane + WAVE, A.dim - 1);
+    for (int s0 = 0; s0 < A.splits; s0 += WAVE) {
+        const int n = min(WAVE, A.splits - s0);
+        const float *ps = p + (int64_t)s0 * w;
+        float f = 0.f, add = 0.f;
+        if (lane < n) {
+            f = __builtin_amdgcn_exp2f(ps[lane * w] - base);
+            add = f * ps[lane * w + 1];
+        }
+#pragma unroll
+        for (int d = 32; d; d /= 2) add += __shfl_xor(add, d);
+        tot += add;
+#pragma unroll 8
+        for (int s = 0; s < n; ++s) {
+            const float fs = __shfl(f, s);
+            a0 += fs * ps[s * w + 2 + e0];
+            a1 += fs * ps[s * w + 2 + e1];
+        }
     }
     const float inv = tot == 0.f ? 0.f : 1.f / tot;
     T *dst = (T *)A.out.ptr + b * A.out.seq + hd * A.out.head;
     if (lane < A.dim) dst[lane] = narrow<T>(a0 * inv);
-    if (lane + 64 < A.dim) dst[lane + 64] = narrow<T>(a1 * inv);
+    if (lane + WAVE < A.dim) dst[lane + WAVE] = narrow<T>(a1 * inv);
     if (lane == 0) A.lse[x] = tot == 0.f ? -INFINITY : mx * LN2 + __logf(tot);
 }
 
@@ -298,12 +318,12 @@ static int check_pages(const spmm_attn_desc_t *a, const spmm_attn_pages_t *p, co
     return SPMM_HIP_OK;
 }
 
-// Blocks that share a sequence's keys: enough for four blocks a compute unit in all, each with SPLIT_MIN keys or more.
+// Blocks that share a sequence's keys: enough for eight blocks a compute unit in all, each with SPLIT_MIN keys or more.
 static int64_t split_count(const spmm_attn_desc_t *a, int64_t max_length) {
     const int64_t group = a->heads / a->kv_heads, base = a->batch * a->kv_heads * ((group + 15) / 16);
     int64_t keys = max_length;
     if (a->window && a->window < keys) keys = (int64_t)a->window + (a->sinks < keys - a->window ? a->sinks : keys - a->window);
-    const int64_t most = (keys + SPLIT_MIN - 1) / SPLIT_MIN, want = base > 0 ? (1024 + base - 1) / base : 1;
+    const int64_t most = (keys + SPLIT_MIN - 1) / SPLIT_MIN, want = base > 0 ? (2048 + base - 1) / base : 1;
     const int64_t n = want < most ? want : most;
     return n < 1 ? 1 : n;
 }
@@ -343,6 +363,9 @@ extern "C" int spmm_attn_paged(const spmm_attn_desc_t *a, const spmm_attn_rows_t
     if (!lse || (uintptr_t)lse % 4) return fail(SPMM_HIP_ERR_ARG, "%s: lse is NULL or not aligned", W);
     if (need > 0 && (!work || (uintptr_t)work % 16 || work_bytes < need))
         return fail(SPMM_HIP_ERR_ARG, "%s: the workspace needs %zu bytes, 16-byte aligned", W, need);
+    // keys are read in pieces of 8 elements, values in pieces of 4 or 8: none may pass the row's end
+    A.k_wide = A.k_wide && a->dim % 8 == 0;
+    A.v_wide = A.v_wide && a->dim % (a->dim <= 64 ? 4 : 8) == 0;
     A.k = (const char *)pages->k;
     A.v = (const char *)pages->v;
     A.pages = pages->pages;
@@ -365,6 +388,7 @@ extern "C" int spmm_attn_paged(const spmm_attn_desc_t *a, const spmm_attn_rows_t
     A.window = a->window;
     A.sinks = a->window ? a->sinks : 0;
     A.splits = (int)split_count(a, max_length);
+    A.page_shift = A.page_rows & (A.page_rows - 1) ? -1 : __builtin_ctzll((unsigned long long)A.page_rows);
     A.scale2 = a->scale * LOG2E;
     A.lse = lse;
     A.part = (float *)work;
