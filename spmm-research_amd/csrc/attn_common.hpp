@@ -50,6 +50,13 @@ __device__ __forceinline__ f32x4 mma16(frag<float> a, frag<float> b, f32x4 c) {
     return c;
 }
 
+// A value that every lane of a wave holds alike, in scalar registers.
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+template <typename T> __device__ __forceinline__ T *uniform(T *p) {
+    const uint64_t x = (uint64_t)p;
+    return (T *)((uint64_t)(uint32_t)uniform((int)x) | (uint64_t)(uint32_t)uniform((int)(x >> 32)) << 32);
+}
+
 // Round to nearest even; the only narrowing in these kernels apart from the stores of results.
 template <typename T> __device__ __forceinline__ T narrow(float x) { return (T)x; }
 
@@ -116,32 +123,59 @@ template <typename T, int DP> struct Tile {
     }
 };
 
-__device__ __align__(16) const uint32_t zero_piece[4] = {0, 0, 0, 0};
+typedef __attribute__((address_space(3))) void lds_void;
+
+// Buffer loads that write LDS: lane l fills the l-th 16 (or 4) bytes from `tile` on with those at byte `off` of the buffer,
+// zeros where that lies outside.  The compiler does not count these loads: LDS is read after arrived<n>() (all of this
+// wave's but the last n are there) and a barrier, and a wave has waited for all before it ends.  (With the builtin
+// it does count them, and waits for every one of them before the next transposing read of any tile.)
+// m0 says where in LDS; a load may read it one wait state after it is written, and scalar registers that a vector
+// instruction wrote (readfirstlane) five after that.  The compiler does not look into the text, so the text waits.
+struct Buffer {
+    typedef int i32x4 __attribute__((ext_vector_type(4)));
+    i32x4 rsrc;
+    __device__ __forceinline__ Buffer(const void *base, int bytes) {
+        const uint64_t b = (uint64_t)base;
+        rsrc = i32x4{uniform((int)b), uniform((int)(b >> 32)) & 0xffff, uniform(bytes), 0x00027000};
+    }
+    static __device__ __forceinline__ int place(const void *tile) { return uniform((int)(uintptr_t)(lds_void *)tile); }
+    __device__ __forceinline__ void to_lds16(void *tile, int off) const {
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(place(tile)), "v"(off), "s"(rsrc) : "memory");
+    }
+    __device__ __forceinline__ void to_lds4(void *tile, int off) const {
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(place(tile)), "v"(off), "s"(rsrc) : "memory");
+    }
+};
+template <int LEFT = 0> __device__ __forceinline__ void arrived() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LEFT) : "memory"); }
 
 // Brings the R rows of a tile from memory to LDS, THREADS threads together.
 template <typename T, int DP, int R, int THREADS> struct Mover {
     using L = Tile<T, DP>;
     static constexpr int PP = L::PITCH / L::EL;             // 16-byte places of a row
-    static constexpr int N = R * PP / THREADS;
-    static_assert(R * PP % THREADS == 0 && THREADS % 64 == 0, "whole waves of pieces");
+    static constexpr int N = R * PP / THREADS, STEP = THREADS / PP;      // loads a thread, rows between them
+    static_assert(R * PP % THREADS == 0 && THREADS % 64 == 0 && STEP > 0, "whole waves of pieces");
+    static constexpr bool SAME = STEP % 16 == 0;            // the exchange within a row repeats every 16 rows
+    int off[SAME ? 1 : N];                                  // byte offset of this thread's pieces from the tile's row 0
 
-    // By the loads that write LDS themselves: lane l of a wave fills place l of 64 consecutive ones, so the exchange of
-    // pieces within a row is in which piece a lane asks for; what is not there comes from a piece of zeros.  Rows are
-    // 16-byte aligned and dim is a multiple of a piece.  row(r): address of the tile's row r, nullptr for zeros.  The
-    // tile is there after arrived() and a barrier.
-    template <typename F> static __device__ __forceinline__ void send(int tid, int dim, T *tile, F row) {
-        typedef __attribute__((address_space(3))) void lds_void;
-        typedef __attribute__((address_space(1))) const void global_void;
+    // By buffer loads that write LDS: lane l of a wave fills place l of 64 consecutive ones, so the exchange of
+    // pieces within a row is in which piece a lane asks for.  The buffer ends with the last row that is there, so what
+    // lies behind it, and the pieces beyond dim, arrive as zeros without a comparison.  Rows are 16-byte aligned, dim
+    // is a multiple of a piece and R rows span less than 2^31 bytes (Rows::direct).
+    __device__ __forceinline__ void start(int tid, int dim, int64_t row) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
+        for (int i = 0; i < (SAME ? 1 : N); ++i) {
             const int p = tid + i * THREADS, r = p / PP, e = ((p % PP) ^ L::swizzle(r)) * L::EL;
-            const T *src = row(r);
-            const void *from = src && e < dim ? (const void *)(src + e) : (const void *)zero_piece;
-            __builtin_amdgcn_global_load_lds((global_void *)from,
-                                             (lds_void *)(tile + (i * THREADS + (tid & ~63)) * L::EL), 16, 0, 0);
+            off[i] = e < dim ? (r * (int)row + e) * (int)sizeof(T) : INT32_MIN;
         }
     }
-    static __device__ __forceinline__ void arrived() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+    // rows: those left from `base` on (uniform).  The tile is there after arrived() and a barrier.
+    __device__ __forceinline__ void send(int wave, T *tile, const T *base, int64_t row, int rows, int dim) const {
+        const int n = min(rows, R);
+        const Buffer buf(base, n > 0 ? ((n - 1) * (int)row + dim) * (int)sizeof(T) : 0);
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            buf.to_lds16(tile + (i * THREADS + wave * 64) * L::EL, SAME ? off[0] + i * STEP * (int)row * (int)sizeof(T) : off[i]);
+    }
 
     // Through registers, element by element: any alignment and width.
     template <typename F> static __device__ __forceinline__ void copy(int tid, int dim, T *tile, F row) {
@@ -229,7 +263,7 @@ struct Seq {
 // Which tile of which sequence is tile number t, `rows` rows of the tiled side (queries or keys) a tile.  Without offsets
 // by division; with offsets every wave sums the tiles of 64 sequences at a time.  Offsets are clamped into the
 // buffers, so bad ones give wrong rows but no access outside.
-__device__ __forceinline__ Seq find_tile(int t, int rows, bool by_key, const int32_t *cu_q, const int32_t *cu_k,
+__device__ __forceinline__ Seq find_tile_any(int t, int rows, bool by_key, const int32_t *cu_q, const int32_t *cu_k,
                                          int64_t batch, int64_t q_len, int64_t k_len) {
     Seq s;
     s.rest = 0;
@@ -267,12 +301,12 @@ __device__ __forceinline__ Seq find_tile(int t, int rows, bool by_key, const int
             const int src = __ffsll(hit) - 1;
             s.b = __builtin_amdgcn_readfirstlane((int)b0 + src);
             s.tile = __builtin_amdgcn_readfirstlane(t - before - __shfl(incl - mine, src));
-            int64_t q0 = min(max((int64_t)cu_q[s.b], (int64_t)0), q_len);
-            int64_t k0 = min(max((int64_t)cu_k[s.b], (int64_t)0), k_len);
-            s.q0 = q0;
-            s.k0 = k0;
-            s.nq = (int)(min(max((int64_t)cu_q[s.b + 1], q0), q_len) - q0);
-            s.nk = (int)(min(max((int64_t)cu_k[s.b + 1], k0), k_len) - k0);
+            const int q0 = (int)min(max((int64_t)cu_q[s.b], (int64_t)0), q_len);
+            const int k0 = (int)min(max((int64_t)cu_k[s.b], (int64_t)0), k_len);
+            s.q0 = __builtin_amdgcn_readfirstlane(q0);
+            s.k0 = __builtin_amdgcn_readfirstlane(k0);
+            s.nq = __builtin_amdgcn_readfirstlane((int)min(max((int64_t)cu_q[s.b + 1], (int64_t)q0), q_len) - q0);
+            s.nk = __builtin_amdgcn_readfirstlane((int)min(max((int64_t)cu_k[s.b + 1], (int64_t)k0), k_len) - k0);
             return s;
         }
         before += __shfl(incl, WAVE - 1);
@@ -288,11 +322,26 @@ __device__ __forceinline__ Seq find_tile(int t, int rows, bool by_key, const int
     return s;
 }
 
+// The same, in scalar registers: what depends on it are then branches and addresses of the whole wave.
+__device__ __forceinline__ Seq find_tile(int t, int rows, bool by_key, const int32_t *cu_q, const int32_t *cu_k,
+                                         int64_t batch, int64_t q_len, int64_t k_len) {
+    Seq s = find_tile_any(t, rows, by_key, cu_q, cu_k, batch, q_len, k_len);
+    s.q0 = uniform((int)s.q0);
+    s.k0 = uniform((int)s.k0);
+    s.nq = uniform(s.nq);
+    s.nk = uniform(s.nk);
+    s.b = uniform(s.b);
+    s.tile = uniform(s.tile);
+    s.rest = uniform((int)s.rest);
+    return s;
+}
+
 // ------------------------------------------------------------------------------------------------ host side
 struct Rows {             // spmm_attn_rows for a kernel
     char *ptr;
     int64_t seq, row, head;
     bool wide;            // 16-byte (inputs) or 4-element (outputs) accesses allowed
+    bool direct;          // wide, rows apart by dim or more, and 128 rows span less than 2^31 bytes
 };
 
 extern thread_local char g_detail[256];

@@ -74,6 +74,7 @@ int check_rows(const spmm_attn_desc_t *a, const spmm_attn_rows_t *r, const char 
     out->wide = (uintptr_t)r->ptr % (el * es) == 0 && a->dim % el == 0;
     for (auto &x : d)
         if (x.count > 1 && x.stride % el) out->wide = false;
+    out->direct = out->wide && r->row >= a->dim && r->row < INT32_MAX / 128 / (int64_t)es;
     return SPMM_HIP_OK;
 }
 

@@ -226,11 +226,14 @@ template <typename T> __global__ __launch_bounds__(64) void paged_join_kernel(Pa
 #pragma unroll
         for (int d = 32; d; d /= 2) add += __shfl_xor(add, d);
         tot += add;
-#pragma unroll 8
-        for (int s = 0; s < n; ++s) {
-            const float fs = __shfl(f, s);
-            a0 += fs * ps[s * w + 2 + e0];
-            a1 += fs * ps[s * w + 2 + e1];
+        for (int s = 0; s < n; s += 8) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {                   // past the last part: its values times 0
+                const float fs = __shfl(f, s + i);
+                const float *pi = ps + min(s + i, n - 1) * w + 2;
+                a0 += fs * pi[e0];
+                a1 += fs * pi[e1];
+            }
         }
     }
     const float inv = tot == 0.f ? 0.f : 1.f / tot;

@@ -12,15 +12,14 @@ namespace attn {
 template <typename T> constexpr int BN_OF = sizeof(T) == 2 ? 64 : 32;      // keys of a tile
 constexpr int BM = 128;                                                      // queries of a workgroup
 
-template <typename T, int DP>
+template <typename T, int DP, bool DIRECT>
 __global__ __launch_bounds__(256, 2) void window_kernel(WindowArgs A) {
     using L = Tile<T, DP>;
     constexpr int BN = BN_OF<T>, ND = DP / 32, NS = DP / 16, NK = BN / 32;
-    __shared__ __align__(16) T sk[2][BN * L::PITCH];
-    __shared__ __align__(16) T sv[2][BN * L::PITCH];
+    __shared__ __align__(16) T sk[2][BN * L::PITCH], sv[2][BN * L::PITCH];
     __shared__ int odd;                              // some staged value of a partly visible tile was not finite
 
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
     int kv, g, t;
     place(A, A.heads / A.kv_heads, &kv, &g, &t);
     t = A.tiles - 1 - t;                             // late queries see more keys: they start first
@@ -64,101 +63,105 @@ __global__ __launch_bounds__(256, 2) void window_kernel(WindowArgs A) {
     const float scale2 = A.scale2 == 0.f ? 1.f : fabsf(A.scale2);
 
     using Move = Mover<T, DP, BN, 256>;
-    const bool direct = A.k.wide && A.v.wide;
-    // keys that no query of the block sees are not read: they may be anything
-    auto key_row = [&](const T *base, const Rows &R, int j) {
-        return j <= pmax && (j >= lo || j < A.mask.sinks) ? base + (int64_t)j * R.row : nullptr;
+    Move mk, mv;
+    if (DIRECT) {
+        mk.start(tid, A.dim, A.k.row);
+        mv.start(tid, A.dim, A.v.row);
+    }
+    auto send = [&](int j0, T *tk, T *tv) {
+        mk.send(wave, tk, kb + (int64_t)j0 * A.k.row, A.k.row, pmax + 1 - j0, A.dim);
+        mv.send(wave, tv, vb + (int64_t)j0 * A.v.row, A.v.row, pmax + 1 - j0, A.dim);
     };
-    auto bring = [&](int j0, int buf, auto how) {
-        how(sk[buf], [&](int r) { return key_row(kb, A.k, j0 + r); });
-        how(sv[buf], [&](int r) { return key_row(vb, A.v, j0 + r); });
-    };
-    auto send = [&](T *tile, auto row) { Move::send(tid, A.dim, tile, row); };
-    auto copy = [&](T *tile, auto row) { Move::copy(tid, A.dim, tile, row); };
     // the tile is in LDS but for a barrier
-    auto settle = [&](int j0, int buf) {
-        if (direct) Move::arrived();
-        else bring(j0, buf, copy);
-        if (!A.mask.all(pmin, pmax, j0, j0 + BN - 1) && Move::any_not_finite(tid, sv[buf])) odd = 1;
+    auto settle = [&](int j0, T *tk, T *tv) {
+        if constexpr (DIRECT) {
+            arrived();
+        } else {
+            auto copy = [&](T *tile, const T *base, int64_t row) {
+                Move::copy(tid, A.dim, tile, [&](int r) { return j0 + r <= pmax ? base + (int64_t)(j0 + r) * row : nullptr; });
+            };
+            copy(tk, kb, A.k.row);
+            copy(tv, vb, A.v.row);
+        }
+        if (!A.mask.all(pmin, pmax, j0, j0 + BN - 1) && Move::any_not_finite(tid, tv)) odd = 1;
     };
 
     f32x16 o[ND];
 #pragma unroll
     for (int d = 0; d < ND; ++d) o[d] = zero16();
     float m = -INFINITY, sum = 0.f;                  // of the scores times scale2
+    auto step = [&](int j0, const T *tk, const T *tv) {
+        if (w0 > w1 || !A.mask.any(w0, w1, j0, j0 + BN - 1)) return;
+        const bool full = A.mask.all(w0, w1, j0, j0 + BN - 1);
+        f32x16 sc[NK];
+#pragma unroll
+        for (int n = 0; n < NK; ++n) {
+            sc[n] = zero16();
+#pragma unroll
+            for (int st = 0; st < NS; ++st)
+                sc[n] = mma32(L::row_frag(tk, n * 32 + (lane & 31), st * 16 + h * 8), qf[st], sc[n]);
+        }
+        if (!full) {
+#pragma unroll
+            for (int n = 0; n < NK; ++n)
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if (!A.mask.sees(p, j0 + n * 32 + row_of(r) + 4 * h)) sc[n][r] = -INFINITY;
+        }
+        float mx = sc[0][0];
+#pragma unroll
+        for (int n = 0; n < NK; ++n)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) mx = fmaxf(mx, sc[n][r]);
+        mx = fmaxf(mx, __shfl_xor(mx, 32));
+        mx = fmaxf(m, mx * scale2);
+        const float base = mx == -INFINITY ? 0.f : mx;
+        if (__any(mx != m)) {
+            const float alpha = __builtin_amdgcn_exp2f(m - base);
+            sum *= alpha;
+#pragma unroll
+            for (int d = 0; d < ND; ++d) o[d] *= alpha;
+            m = mx;
+        }
+#pragma unroll
+        for (int n = 0; n < NK; ++n)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                sc[n][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[n][r], scale2, -base));
+                sum += sc[n][r];
+            }
+        const bool careful = !full && __builtin_amdgcn_readfirstlane(odd);
+        if (!careful) {
+#pragma unroll
+            for (int n = 0; n < NK; ++n)
+#pragma unroll
+                for (int k2 = 0; k2 < 2; ++k2) {
+                    const frag<T> pf = next_operand<T>(sc[n], k2);
+#pragma unroll
+                    for (int d = 0; d < ND; ++d)
+                        o[d] = mma32(L::col_frag(tv, n * 32 + k2 * 16, d * 32, lane), pf, o[d]);
+                }
+        } else {
+            Careful<T, DP, BN> c;
+            for (int d = 0; d < ND; ++d) c.acc[d] = o[d];
+            for (int n = 0; n < NK; ++n) c.w[n] = sc[n];
+            careful_product<T, DP, BN>(&c, tv, lane, A.mask, p, j0, true, INT32_MAX);
+            for (int d = 0; d < ND; ++d) o[d] = c.acc[d];
+        }
+    };
+
     __syncthreads();                                 // `odd` is set
     if (tiles) {
-        if (direct) bring(tile_at(0), 0, send);
-        settle(tile_at(0), 0);
+        if (DIRECT) send(tile_at(0), sk[0], sv[0]);
+        settle(tile_at(0), sk[0], sv[0]);
     }
     __syncthreads();
-    for (int it = 0; it < tiles; ++it) {
-        const int j0 = tile_at(it), buf = it & 1;
-        if (direct && it + 1 < tiles) bring(tile_at(it + 1), buf ^ 1, send);
-        if (w0 <= w1 && A.mask.any(w0, w1, j0, j0 + BN - 1)) {
-            const bool full = A.mask.all(w0, w1, j0, j0 + BN - 1);
-            f32x16 sc[NK];
-#pragma unroll
-            for (int n = 0; n < NK; ++n) {
-                sc[n] = zero16();
-#pragma unroll
-                for (int st = 0; st < NS; ++st)
-                    sc[n] = mma32(L::row_frag(sk[buf], n * 32 + (lane & 31), st * 16 + h * 8), qf[st], sc[n]);
-            }
-            if (!full) {
-#pragma unroll
-                for (int n = 0; n < NK; ++n)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r)
-                        if (!A.mask.sees(p, j0 + n * 32 + row_of(r) + 4 * h)) sc[n][r] = -INFINITY;
-            }
-            float mx = sc[0][0];
-#pragma unroll
-            for (int n = 0; n < NK; ++n)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) mx = fmaxf(mx, sc[n][r]);
-            mx = fmaxf(mx, __shfl_xor(mx, 32));
-            mx = fmaxf(m, mx * scale2);
-            const float base = mx == -INFINITY ? 0.f : mx;
-            if (__any(mx != m)) {
-                const float alpha = __builtin_amdgcn_exp2f(m - base);
-                sum *= alpha;
-#pragma unroll
-                for (int d = 0; d < ND; ++d) o[d] *= alpha;
-                m = mx;
-            }
-#pragma unroll
-            for (int n = 0; n < NK; ++n)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    sc[n][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[n][r], scale2, -base));
-                    sum += sc[n][r];
-                }
-            const bool careful = !full && __builtin_amdgcn_readfirstlane(odd);
-            if (!careful) {
-#pragma unroll
-                for (int n = 0; n < NK; ++n)
-#pragma unroll
-                    for (int k2 = 0; k2 < 2; ++k2) {
-                        const frag<T> pf = next_operand<T>(sc[n], k2);
-#pragma unroll
-                        for (int d = 0; d < ND; ++d)
-                            o[d] = mma32(L::col_frag(sv[buf], n * 32 + k2 * 16, d * 32, lane), pf, o[d]);
-                    }
-            } else {
-#pragma unroll
-                for (int n = 0; n < NK; ++n)
-#pragma unroll
-                    for (int k2 = 0; k2 < 2; ++k2) {
-                        const frag<T> pf = next_operand<T>(sc[n], k2);
-#pragma unroll
-                        for (int d = 0; d < ND; ++d)
-                            o[d] = mma32(only_finite<T>(L::col_frag(sv[buf], n * 32 + k2 * 16, d * 32, lane)), pf, o[d]);
-                    }
-                add_not_finite<T, DP>(o, sv[buf], BN, lane, [&](int r) { return A.mask.sees(p, j0 + r); });
-            }
-        }
-        if (it + 1 < tiles) settle(tile_at(it + 1), buf ^ 1);
+    for (int it = 0; it < tiles; ++it) {             // a tile's loads are under way while the one before it is used
+        const int buf = it & 1;
+        const bool more = it + 1 < tiles;
+        if (DIRECT && more) send(tile_at(it + 1), sk[buf ^ 1], sv[buf ^ 1]);
+        step(tile_at(it), sk[buf], sv[buf]);
+        if (more) settle(tile_at(it + 1), sk[buf ^ 1], sv[buf ^ 1]);
         __syncthreads();
     }
     sum += __shfl_xor(sum, 32);
@@ -207,9 +210,12 @@ int tile_count(const spmm_attn_desc_t *a, const char *where, bool packed, int64_
     return SPMM_HIP_OK;
 }
 
-template <typename T> static const void *window_of(int dim) {
-    return dim <= 64 ? (const void *)window_kernel<T, 64> : dim <= 96 ? (const void *)window_kernel<T, 96>
-                                                                      : (const void *)window_kernel<T, 128>;
+template <typename T, bool DIRECT> static const void *window_by(int dim) {
+    return dim <= 64 ? (const void *)window_kernel<T, 64, DIRECT> : dim <= 96 ? (const void *)window_kernel<T, 96, DIRECT>
+                                                                              : (const void *)window_kernel<T, 128, DIRECT>;
+}
+template <typename T> static const void *window_of(int dim, bool direct) {
+    return direct ? window_by<T, true>(dim) : window_by<T, false>(dim);
 }
 
 }  // namespace attn
@@ -237,8 +243,9 @@ extern "C" int spmm_attn_window(const spmm_attn_desc_t *a, const spmm_attn_rows_
     if ((st = tile_count(a, W, packed, a->q_len, BM, &A.tiles))) return st;
     OnDevice on(a->device, W);
     if (on.status) return on.status;
-    const void *kern = a->dtype == SPMM_ATTN_F32 ? window_of<float>(a->dim)
-                       : a->dtype == SPMM_ATTN_F16 ? window_of<_Float16>(a->dim) : window_of<__bf16>(a->dim);
+    const bool direct = A.k.direct && A.v.direct;
+    const void *kern = a->dtype == SPMM_ATTN_F32 ? window_of<float>(a->dim, direct)
+                       : a->dtype == SPMM_ATTN_F16 ? window_of<_Float16>(a->dim, direct) : window_of<__bf16>(a->dim, direct);
     void *args[] = {&A};
     return launch(kern, W, (int64_t)A.tiles * a->heads, 256, args, stream);
 }

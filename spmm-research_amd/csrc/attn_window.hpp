@@ -7,13 +7,15 @@ namespace attn {
 struct WindowArgs {
     Rows q, k, v, out, dout, dq, dk, dv;
     float *lse;              // forward: written; gradients: read
-    float *delta;            // gradients: sum_d dout * out of every query row, laid out like lse
+    float *stats;            // gradients: of every query row, laid out like lse, lse in powers of two and sum_d dout * out
     const int32_t *cu_q, *cu_k;
     int64_t batch, q_len, k_len;
     int heads, kv_heads, dim;
     Mask mask;
     float scale, scale2;     // scale2 = scale * log2(e): the exponentials are powers of two
     int tiles, zero_rest;
+    float *part;             // gradients: parts of the first keys' gradients
+    int chunk;               // queries of a part, 0: not split
 };
 
 // Key head, query head inside its group, and tile of a block.  Consecutive blocks go round the eight dies, so
@@ -41,28 +43,49 @@ template <typename T> __device__ void zero_rows(const Rows &r, int64_t from, int
         }
 }
 
-// acc[d][r] += the tile's values that are not finite and stand in a row that the lane's column sees.  A masked place
-// enters the matrix instructions as 0 * x, which is NaN for such an x: it is taken out of the operand (only_finite)
-// and put back here where it is seen.
-template <typename T, int DP, typename F>
-__device__ __forceinline__ void add_not_finite(f32x16 (&acc)[DP / 32], const T *tile, int rows, int lane, F sees) {
+// row of register r (+ 4 h) in a 32x32 product
+__device__ __forceinline__ constexpr int row_of(int r) { return 8 * (r >> 2) + (r & 3); }
+
+template <typename T> __device__ __forceinline__ frag<T> next_operand(const f32x16 &c, int ks);
+
+// acc += tile^T w over a tile of ROWS rows some value of which is not finite; w: weights of the tile's rows for the lane's
+// column, 0 where seen(row) does not hold.  A masked place enters the matrix instructions as 0 * x, which is NaN for such
+// an x: it is taken out of the operand and put back where it is seen.  Rare, so a function of its own that takes no
+// registers from the loops that call it.
+template <typename T, int DP, int ROWS> struct Careful {
+    f32x16 acc[DP / 32], w[ROWS / 32];
+};
+template <typename T, int DP, int ROWS>
+__device__ __attribute__((noinline)) void careful_product(Careful<T, DP, ROWS> *c, const T *tile, int lane, Mask mask, int p, int j0,
+                                                          bool by_key, int last) {
 #pragma unroll 1
-    for (int rr = 0; rr < rows; ++rr) {
-        const bool seen = sees(rr);
+    for (int n = 0; n < ROWS / 32; ++n)
+#pragma unroll 1
+        for (int k2 = 0; k2 < 2; ++k2) {
+            frag<T> pf;
 #pragma unroll
-        for (int dt = 0; dt < DP / 32; ++dt)
+            for (int j = 0; j < 8; ++j) pf[j] = narrow<T>(c->w[n][8 * k2 + j]);
+#pragma unroll 1
+            for (int d = 0; d < DP / 32; ++d) {
+                frag<T> f = Tile<T, DP>::col_frag(tile, n * 32 + k2 * 16, d * 32, lane);
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (!finite_f((float)f[j])) f[j] = (T)0.f;
+                c->acc[d] = mma32(f, pf, c->acc[d]);
+            }
+        }
+#pragma unroll 1
+    for (int rr = 0; rr < ROWS; ++rr) {
+        // rows are keys and the column a query at p, or rows are queries at j0 + rr and the column key p
+        const bool seen = j0 + rr <= last && (by_key ? mask.sees(p, j0 + rr) : mask.sees(j0 + rr, p));
+#pragma unroll 1
+        for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                const float x = (float)tile[Tile<T, DP>::at(rr, dt * 32 + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3))];
-                if (seen && !finite_f(x)) acc[dt][r] += x;
+                const float x = (float)tile[Tile<T, DP>::at(rr, d * 32 + 8 * (r >> 2) + (r & 3) + 4 * (lane >> 5))];
+                if (seen && !finite_f(x)) c->acc[d][r] += x;
             }
     }
-}
-template <typename T> __device__ __forceinline__ frag<T> only_finite(frag<T> f) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-        if (!finite_f((float)f[j])) f[j] = (T)0.f;
-    return f;
 }
 
 // registers 8 ks .. 8 ks + 7 of a product as the next product's operand (rows 16 ks + ... in col_frag's order)
@@ -79,9 +102,6 @@ __device__ __forceinline__ f32x16 zero16() {
     for (int r = 0; r < 16; ++r) z[r] = 0.f;
     return z;
 }
-// row of register r (+ 4 h) in a 32x32 product
-__device__ __forceinline__ constexpr int row_of(int r) { return 8 * (r >> 2) + (r & 3); }
-
 int window_args(const spmm_attn_desc_t *a, const char *where, const int32_t *cu_q, const int32_t *cu_k, WindowArgs *out);
 int tile_count(const spmm_attn_desc_t *a, const char *where, bool packed, int64_t len, int rows, int *tiles);
 

@@ -10,7 +10,8 @@
 
 namespace attn {
 
-// D of 16 rows x heads a block: 16 lanes a row, 8 elements a lane.
+// What the two kernels below need of every query row, 16 rows x heads a block, 16 lanes a row, 8 elements a lane:
+// lse in powers of two (+inf where the query sees nothing: every weight is then exp2(x - inf) = 0), and D.
 template <typename T> __global__ __launch_bounds__(256) void delta_kernel(WindowArgs A) {
     const bool packed = A.cu_q != nullptr;
     const int64_t rows = (packed ? 1 : A.batch) * A.q_len, x = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
@@ -25,20 +26,23 @@ template <typename T> __global__ __launch_bounds__(256) void delta_kernel(Window
     for (int j = 0; j < 8; ++j) s += (float)o[j] * (float)d[j];
 #pragma unroll
     for (int w = 8; w; w /= 2) s += __shfl_xor(s, w);
-    if (mine && (threadIdx.x & 15) == 0) A.delta[x] = s;
+    if (mine && (threadIdx.x & 15) == 0) {
+        const float l = A.lse[x];
+        A.stats[2 * x] = l == -INFINITY ? INFINITY : l * LOG2E;
+        A.stats[2 * x + 1] = s;
+    }
 }
 
 constexpr int GM = 128;                      // rows a workgroup owns, 32 a wave
 constexpr int GN = 32;                       // rows of a staged tile
 
-template <typename T, int DP>
+template <typename T, int DP, bool DIRECT>
 __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void grad_q_kernel(WindowArgs A) {
     using L = Tile<T, DP>;
     constexpr int ND = DP / 32, NS = DP / 16;
-    __shared__ __align__(16) T sk[2][GN * L::PITCH];
-    __shared__ __align__(16) T sv[2][GN * L::PITCH];
+    __shared__ __align__(16) T sk[2][GN * L::PITCH], sv[2][GN * L::PITCH];
     __shared__ int odd;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
+    const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), h = lane >> 5;
     int kv, g, t;
     place(A, A.heads / A.kv_heads, &kv, &g, &t);
     t = A.tiles - 1 - t;
@@ -75,64 +79,81 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void grad_q_kernel(Win
         }
         if (mine) {
             const int64_t x = (packed ? s.q0 + i : s.b * A.q_len + i) * A.heads + head;
-            lse2 = A.lse[x] == -INFINITY ? INFINITY : A.lse[x] * LOG2E;
-            delta = A.delta[x];
+            lse2 = A.stats[2 * x];
+            delta = A.stats[2 * x + 1];
         }
     }
     using Move = Mover<T, DP, GN, 256>;
-    const bool direct = A.k.wide && A.v.wide;
-    auto key_row = [&](const T *base, const Rows &R, int j) {
-        return j <= pmax && (j >= lo || j < A.mask.sinks) ? base + (int64_t)j * R.row : nullptr;
+    Move mk, mv;
+    if (DIRECT) {
+        mk.start(tid, A.dim, A.k.row);
+        mv.start(tid, A.dim, A.v.row);
+    }
+    auto send = [&](int j0, T *tk, T *tv) {
+        mk.send(wave, tk, kb + (int64_t)j0 * A.k.row, A.k.row, pmax + 1 - j0, A.dim);
+        mv.send(wave, tv, vb + (int64_t)j0 * A.v.row, A.v.row, pmax + 1 - j0, A.dim);
     };
-    auto bring = [&](int j0, int buf, auto how) {
-        how(sk[buf], [&](int r) { return key_row(kb, A.k, j0 + r); });
-        how(sv[buf], [&](int r) { return key_row(vb, A.v, j0 + r); });
-    };
-    auto send = [&](T *tile, auto row) { Move::send(tid, A.dim, tile, row); };
-    auto copy = [&](T *tile, auto row) { Move::copy(tid, A.dim, tile, row); };
-    auto settle = [&](int j0, int buf) {
-        if (direct) Move::arrived();
-        else bring(j0, buf, copy);
-        if (!A.mask.all(pmin, pmax, j0, j0 + GN - 1) && Move::any_not_finite(tid, sk[buf])) odd = 1;
+    auto settle = [&](int j0, T *tk, T *tv) {
+        if constexpr (DIRECT) {
+            arrived();
+        } else {
+            auto copy = [&](T *tile, const T *base, int64_t row) {
+                Move::copy(tid, A.dim, tile, [&](int r) { return j0 + r <= pmax ? base + (int64_t)(j0 + r) * row : nullptr; });
+            };
+            copy(tk, kb, A.k.row);
+            copy(tv, vb, A.v.row);
+        }
+        if (!A.mask.all(pmin, pmax, j0, j0 + GN - 1) && Move::any_not_finite(tid, tk)) odd = 1;
     };
     f32x16 dq[ND];
 #pragma unroll
     for (int d = 0; d < ND; ++d) dq[d] = zero16();
-    __syncthreads();
-    if (tiles) {
-        if (direct) bring(tile_at(0), 0, send);
-        settle(tile_at(0), 0);
-    }
-    __syncthreads();
-    for (int it = 0; it < tiles; ++it) {
-        const int j0 = tile_at(it), buf = it & 1;
-        if (direct && it + 1 < tiles) bring(tile_at(it + 1), buf ^ 1, send);
-        if (w0 <= w1 && A.mask.any(w0, w1, j0, j0 + GN - 1)) {
-            const bool full = A.mask.all(w0, w1, j0, j0 + GN - 1);
-            f32x16 sc = zero16(), dp = zero16();
+    auto step = [&](int j0, const T *tk, const T *tv) {
+        if (w0 > w1 || !A.mask.any(w0, w1, j0, j0 + GN - 1)) return;
+        const bool full = A.mask.all(w0, w1, j0, j0 + GN - 1);
+        f32x16 sc = zero16(), dp = zero16();
 #pragma unroll
-            for (int st = 0; st < NS; ++st) {
-                sc = mma32(L::row_frag(sk[buf], lane & 31, st * 16 + h * 8), qf[st], sc);
-                dp = mma32(L::row_frag(sv[buf], lane & 31, st * 16 + h * 8), df[st], dp);
-            }
+        for (int st = 0; st < NS; ++st) {
+            sc = mma32(L::row_frag(tk, lane & 31, st * 16 + h * 8), qf[st], sc);
+            dp = mma32(L::row_frag(tv, lane & 31, st * 16 + h * 8), df[st], dp);
+        }
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const float ds = __builtin_amdgcn_exp2f(sc[r] * A.scale2 - lse2) * (dp[r] - delta);
-                sc[r] = full || A.mask.sees(p, j0 + row_of(r) + 4 * h) ? ds : 0.f;
-            }
-            const bool careful = !full && __builtin_amdgcn_readfirstlane(odd);      // a seen key that is not finite has made the whole row NaN already
+        for (int r = 0; r < 16; ++r)
+            sc[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[r], A.scale2, -lse2)) * (dp[r] - delta);
+        if (!full) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                if (!A.mask.sees(p, j0 + row_of(r) + 4 * h)) sc[r] = 0.f;
+        }
+        // a seen key that is not finite makes the row's weights NaN, so it need not be put back
+        const bool careful = !full && uniform(odd);
+        if (!careful) {
 #pragma unroll
             for (int k2 = 0; k2 < 2; ++k2) {
                 const frag<T> dsf = next_operand<T>(sc, k2);
 #pragma unroll
-                for (int d = 0; d < ND; ++d) {
-                    frag<T> kf = L::col_frag(sk[buf], k2 * 16, d * 32, lane);
-                    if (careful) kf = only_finite<T>(kf);
-                    dq[d] = mma32(kf, dsf, dq[d]);
-                }
+                for (int d = 0; d < ND; ++d) dq[d] = mma32(L::col_frag(tk, k2 * 16, d * 32, lane), dsf, dq[d]);
             }
+        } else {
+            Careful<T, DP, GN> c;
+            for (int d = 0; d < ND; ++d) c.acc[d] = dq[d];
+            c.w[0] = sc;
+            careful_product<T, DP, GN>(&c, tk, lane, A.mask, p, j0, true, -1);
+            for (int d = 0; d < ND; ++d) dq[d] = c.acc[d];
         }
-        if (it + 1 < tiles) settle(tile_at(it + 1), buf ^ 1);
+    };
+    __syncthreads();
+    if (tiles) {
+        if (DIRECT) send(tile_at(0), sk[0], sv[0]);
+        settle(tile_at(0), sk[0], sv[0]);
+    }
+    __syncthreads();
+    for (int it = 0; it < tiles; ++it) {
+        const int buf = it & 1;
+        const bool more = it + 1 < tiles;
+        if (DIRECT && more) send(tile_at(it + 1), sk[buf ^ 1], sv[buf ^ 1]);
+        step(tile_at(it), sk[buf], sv[buf]);
+        if (more) settle(tile_at(it + 1), sk[buf ^ 1], sv[buf ^ 1]);
         __syncthreads();
     }
     if (!mine) return;
@@ -145,21 +166,39 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void grad_q_kernel(Win
                       f32x4{dq[d][r] * A.scale, dq[d][r + 1] * A.scale, dq[d][r + 2] * A.scale, dq[d][r + 3] * A.scale});
 }
 
-template <typename T, int DP>
+// The first keys that stay visible are seen by every later query, the others by a window of them: were their block to
+// take all its queries, it would be many times the others' length and the last to end.  So with few of them (A.chunk > 0)
+// their block takes its window's queries only, further blocks take chunks of the other queries each, and what
+// they find for these keys goes to `part` in 32 bits and is summed in order by join_kernel.
+__device__ __forceinline__ float *part_of(const WindowArgs &A, int64_t slot, int kv) {
+    return A.part + (slot * A.kv_heads + kv) * 2 * A.mask.sinks * A.dim;
+}
+__device__ __forceinline__ int64_t chunk_slot(const WindowArgs &A, const Seq &s, bool packed, int c) {
+    return A.batch + (packed ? s.q0 / A.chunk + s.b : s.b * ((A.q_len + A.chunk - 1) / A.chunk)) + c;
+}
+// last query that sees one of the keys n0 .. n1 through the window
+__device__ __forceinline__ int window_end(const WindowArgs &A, const Seq &s, int n1) {
+    return min(s.nq - 1, n1 + A.mask.window - 1 - (s.nk - s.nq));
+}
+
+constexpr int STAGES = 4;                    // tiles of queries on their way or in use
+
+template <typename T, int DP, bool DIRECT>
 __global__ __launch_bounds__(256, 1) void grad_kv_kernel(WindowArgs A) {
     using L = Tile<T, DP>;
     constexpr int ND = DP / 32, NS = DP / 16;
-    __shared__ __align__(16) T sq[2][GN * L::PITCH];
-    __shared__ __align__(16) T sd[2][GN * L::PITCH];
-    __shared__ __align__(16) float slse[2][GN], sdelta[2][GN];
+    __shared__ __align__(16) T sq[STAGES][GN * L::PITCH], sd[STAGES][GN * L::PITCH];
+    __shared__ __align__(16) float ss[STAGES][2 * GN];              // lse and D of the tile's rows
     __shared__ int odd;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
+    const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), h = lane >> 5;
     int kv, g, t;
     place(A, 1, &kv, &g, &t);
     const bool packed = A.cu_q != nullptr;
-    const Seq s = find_tile(t, GM, true, A.cu_q, A.cu_k, A.batch, A.q_len, A.k_len);
+    const bool extra = t >= A.tiles;                                 // a chunk of queries for the first keys
+    const Seq s = extra ? find_tile(t - A.tiles, A.chunk, false, A.cu_q, A.cu_k, A.batch, A.q_len, A.k_len)
+                        : find_tile(t, GM, true, A.cu_q, A.cu_k, A.batch, A.q_len, A.k_len);
     if (s.tile < 0) {
-        if (A.zero_rest && packed) {
+        if (A.zero_rest && packed && !extra) {
             const int64_t from = s.rest + (int64_t)(t - s.nq) * GM, step = (int64_t)(A.tiles - s.nq) * GM;
             zero_rows<T>(A.dk, from, step, GM, A.k_len, kv, A.dim);
             zero_rows<T>(A.dv, from, step, GM, A.k_len, kv, A.dim);
@@ -168,14 +207,21 @@ __global__ __launch_bounds__(256, 1) void grad_kv_kernel(WindowArgs A) {
     }
     if (tid == 0) odd = 0;
     const int group = A.heads / A.kv_heads;
-    const int shift = s.nk - s.nq, n0 = s.tile * GM, n1 = min(n0 + GM, s.nk) - 1;
+    const int shift = s.nk - s.nq, n0 = extra ? 0 : s.tile * GM;
+    const int n1 = min(n0 + GM, extra ? min(A.mask.sinks, s.nk) : s.nk) - 1;
+    const bool first = A.chunk > 0 && n0 < A.mask.sinks;            // the first keys' results go to `part`
     // queries that see some key of the block
-    const int i0 = max(0, n0 - shift);
-    const int i1 = A.mask.window == 0 || n0 < A.mask.sinks ? s.nq - 1 : min(s.nq - 1, n1 + A.mask.window - 1 - shift);
+    int i0 = max(0, n0 - shift);
+    int i1 = A.mask.window == 0 || (n0 < A.mask.sinks && !first) ? s.nq - 1 : window_end(A, s, n1);
+    if (extra) {
+        i0 = max(s.tile * A.chunk, window_end(A, s, min(GM, s.nk) - 1) + 1);
+        i1 = min((s.tile + 1) * A.chunk, s.nq) - 1;
+        if (i1 < i0 || n1 < 0) return;
+    }
     const int q0t = i0 / GN, nqt = i1 >= i0 ? i1 / GN - q0t + 1 : 0, tiles = nqt * group;
 
     const int key = n0 + wave * 32 + (lane & 31);
-    const bool mine = key < s.nk;
+    const bool mine = key <= n1;
     const int c0 = n0 + wave * 32, c1 = min(c0 + 31, n1);          // the wave's keys
     frag<T> kf[NS], vf[NS];
     {
@@ -188,93 +234,116 @@ __global__ __launch_bounds__(256, 1) void grad_kv_kernel(WindowArgs A) {
         }
     }
     using Move = Mover<T, DP, GN, 256>;
-    const bool direct = A.q.wide && A.dout.wide;
-    auto live = [&](int i) { return i >= i0 && i <= i1; };
-    auto bring = [&](int it, int buf, auto how) {
+    constexpr int LOADS = 2 * Move::N + 1;                           // of a tile, a wave
+    Move mq, md;
+    if (DIRECT) {
+        mq.start(tid, A.dim, A.q.row);
+        md.start(tid, A.dim, A.dout.row);
+    }
+    const float *stats = A.stats + (packed ? s.q0 : s.b * A.q_len) * A.heads * 2;
+    // tile `it`: query tile q0t + it % nqt of the group's head it / nqt; beyond the last there are no rows
+    auto send = [&](int it, int buf) {
+        const int head = kv * group + min(it / max(nqt, 1), group - 1), j0 = (q0t + it % max(nqt, 1)) * GN;
+        const int rows = it < tiles ? s.nq - j0 : 0;
+        mq.send(wave, sq[buf], seq_base<T>(A.q, s, s.q0, packed, head) + (int64_t)j0 * A.q.row, A.q.row, rows, A.dim);
+        md.send(wave, sd[buf], seq_base<T>(A.dout, s, s.q0, packed, head) + (int64_t)j0 * A.dout.row, A.dout.row, rows, A.dim);
+        const int n = min(rows, GN);
+        const Buffer b(stats + ((int64_t)j0 * A.heads + head) * 2, n > 0 ? ((n - 1) * A.heads + 1) * 8 : 0);
+        b.to_lds4(ss[buf], (lane >> 1) * A.heads * 8 + (lane & 1) * 4);     // every wave alike: equal counts of loads
+    };
+    auto copy = [&](int it, int buf) {
         const int head = kv * group + it / nqt, j0 = (q0t + it % nqt) * GN;
         const T *qb = seq_base<T>(A.q, s, s.q0, packed, head), *db = seq_base<T>(A.dout, s, s.q0, packed, head);
-        how(sq[buf], [&](int r) { return live(j0 + r) ? qb + (int64_t)(j0 + r) * A.q.row : nullptr; });
-        how(sd[buf], [&](int r) { return live(j0 + r) ? db + (int64_t)(j0 + r) * A.dout.row : nullptr; });
-    };
-    float stat = 0.f;                                // lse or delta of one of the tile's rows, on its way to LDS
-    auto load_stat = [&](int it) {
-        if (tid >= 2 * GN) return;
-        const int head = kv * group + it / nqt, i = (q0t + it % nqt) * GN + tid % GN;
-        const int64_t x = ((packed ? s.q0 : s.b * A.q_len) + i) * A.heads + head;
-        stat = tid < GN ? INFINITY : 0.f;            // no row, or one that sees nothing: P = exp2(x - inf) = 0
-        if (!live(i)) return;
-        if (tid >= GN) stat = A.delta[x];
-        else if (A.lse[x] != -INFINITY) stat = A.lse[x] * LOG2E;
-    };
-    auto send = [&](T *tile, auto row) { Move::send(tid, A.dim, tile, row); };
-    auto copy = [&](T *tile, auto row) { Move::copy(tid, A.dim, tile, row); };
-    auto settle = [&](int it, int buf) {
-        const int p0 = (q0t + it % nqt) * GN + shift;
-        if (direct) Move::arrived();
-        else bring(it, buf, copy);
-        if (!A.mask.all(p0, p0 + GN - 1, n0, n1) &&
-            (Move::any_not_finite(tid, sq[buf]) || Move::any_not_finite(tid, sd[buf]))) odd = 1;
-        if (tid < GN) slse[buf][tid] = stat;
-        else if (tid < 2 * GN) sdelta[buf][tid - GN] = stat;
+        Move::copy(tid, A.dim, sq[buf], [&](int r) { return j0 + r < s.nq ? qb + (int64_t)(j0 + r) * A.q.row : nullptr; });
+        Move::copy(tid, A.dim, sd[buf], [&](int r) { return j0 + r < s.nq ? db + (int64_t)(j0 + r) * A.dout.row : nullptr; });
+        if (tid < 2 * GN) ss[buf][tid] = j0 + tid / 2 < s.nq ? stats[((int64_t)(j0 + tid / 2) * A.heads + head) * 2 + tid % 2] : 0.f;
     };
     f32x16 dk[ND], dv[ND];
 #pragma unroll
     for (int d = 0; d < ND; ++d) dk[d] = dv[d] = zero16();
-    __syncthreads();
-    if (tiles) {
-        load_stat(0);
-        if (direct) bring(0, 0, send);
-        settle(0, 0);
-    }
-    __syncthreads();
-    for (int it = 0; it < tiles; ++it) {
-        const int j0 = (q0t + it % nqt) * GN, p0 = j0 + shift, buf = it & 1;
-        if (it + 1 < tiles) {
-            load_stat(it + 1);
-            if (direct) bring(it + 1, buf ^ 1, send);
+    // rows behind the last query are zeros, lse and D too: P = 1 then, and adds 1 * 0
+    auto step = [&](int j0, const T *tq, const T *td, const float *ts) {
+        const int p0 = j0 + shift;
+        if (c0 > c1 || !A.mask.any(p0, p0 + GN - 1, c0, c1)) return;
+        const bool full = A.mask.all(p0, p0 + GN - 1, c0, c1) && j0 >= i0 && j0 + GN - 1 <= i1;
+        f32x16 sc = zero16(), dp = zero16();
+#pragma unroll
+        for (int st = 0; st < NS; ++st) {
+            sc = mma32(L::row_frag(tq, lane & 31, st * 16 + h * 8), kf[st], sc);
+            dp = mma32(L::row_frag(td, lane & 31, st * 16 + h * 8), vf[st], dp);
         }
-        if (c0 <= c1 && A.mask.any(p0, p0 + GN - 1, c0, c1)) {
-            const bool full = A.mask.all(p0, p0 + GN - 1, c0, c1);
-            f32x16 sc = zero16(), dp = zero16();
 #pragma unroll
-            for (int st = 0; st < NS; ++st) {
-                sc = mma32(L::row_frag(sq[buf], lane & 31, st * 16 + h * 8), kf[st], sc);
-                dp = mma32(L::row_frag(sd[buf], lane & 31, st * 16 + h * 8), vf[st], dp);
+        for (int r2 = 0; r2 < 16; r2 += 2) {
+            const f32x4 st = *reinterpret_cast<const f32x4 *>(ts + 2 * (row_of(r2) + 4 * h));
+#pragma unroll
+            for (int r = r2; r < r2 + 2; ++r) {
+                sc[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[r], A.scale2, -st[2 * (r - r2)]));
+                dp[r] = sc[r] * (dp[r] - st[2 * (r - r2) + 1]);
             }
+        }
+        if (!full) {
 #pragma unroll
-            for (int r4 = 0; r4 < 16; r4 += 4) {
-                const f32x4 l4 = *reinterpret_cast<const f32x4 *>(&slse[buf][row_of(r4) + 4 * h]);
-                const f32x4 d4 = *reinterpret_cast<const f32x4 *>(&sdelta[buf][row_of(r4) + 4 * h]);
-#pragma unroll
-                for (int r = r4; r < r4 + 4; ++r) {
-                    const bool seen = full || A.mask.sees(p0 + row_of(r) + 4 * h, key);
-                    const float pr = __builtin_amdgcn_exp2f(sc[r] * A.scale2 - l4[r - r4]);
-                    dp[r] = seen ? pr * (dp[r] - d4[r - r4]) : 0.f;
-                    sc[r] = seen ? pr : 0.f;
-                }
+            for (int r = 0; r < 16; ++r) {
+                const int i = j0 + row_of(r) + 4 * h;
+                if (i < i0 || i > i1 || !A.mask.sees(i + shift, key)) sc[r] = dp[r] = 0.f;
             }
-            const bool careful = !full && __builtin_amdgcn_readfirstlane(odd);
+        }
+        const bool careful = !full && uniform(odd);
+        if (!careful) {
 #pragma unroll
             for (int k2 = 0; k2 < 2; ++k2) {
                 const frag<T> pf = next_operand<T>(sc, k2), dsf = next_operand<T>(dp, k2);
 #pragma unroll
                 for (int d = 0; d < ND; ++d) {
-                    frag<T> of = L::col_frag(sd[buf], k2 * 16, d * 32, lane), qf = L::col_frag(sq[buf], k2 * 16, d * 32, lane);
-                    if (careful) {
-                        of = only_finite<T>(of);
-                        qf = only_finite<T>(qf);     // a query that is not finite has an lse that is not, so NaN in dsf
-                    }
-                    dv[d] = mma32(of, pf, dv[d]);
-                    dk[d] = mma32(qf, dsf, dk[d]);
+                    dv[d] = mma32(L::col_frag(td, k2 * 16, d * 32, lane), pf, dv[d]);
+                    dk[d] = mma32(L::col_frag(tq, k2 * 16, d * 32, lane), dsf, dk[d]);
                 }
             }
-            if (careful)
-                add_not_finite<T, DP>(dv, sd[buf], GN, lane, [&](int r) { return j0 + r <= i1 && A.mask.sees(p0 + r, key); });
+        } else {
+            // a query that is not finite has an lse that is not, so its weights are NaN: it need not be put back
+            Careful<T, DP, GN> c;
+            for (int d = 0; d < ND; ++d) c.acc[d] = dv[d];
+            c.w[0] = sc;
+            careful_product<T, DP, GN>(&c, td, lane, A.mask, key, p0, false, i1 + shift);
+            for (int d = 0; d < ND; ++d) dv[d] = c.acc[d];
+            for (int d = 0; d < ND; ++d) c.acc[d] = dk[d];
+            c.w[0] = dp;
+            careful_product<T, DP, GN>(&c, tq, lane, A.mask, key, p0, false, INT32_MIN);
+            for (int d = 0; d < ND; ++d) dk[d] = c.acc[d];
         }
-        if (it + 1 < tiles) settle(it + 1, buf ^ 1);
-        __syncthreads();
+    };
+    __syncthreads();
+    if (DIRECT) {
+#pragma unroll
+        for (int it = 0; it < STAGES - 1; ++it) send(it, it);
     }
+    for (int it = 0; it < tiles; ++it) {
+        const int buf = it % STAGES, j0 = (q0t + it % nqt) * GN, p0 = j0 + shift;
+        if (DIRECT) arrived<(STAGES - 2) * LOADS>();
+        else copy(it, buf);
+        if (!(A.mask.all(p0, p0 + GN - 1, n0, n1) && j0 >= i0 && j0 + GN - 1 <= i1) &&
+            (Move::any_not_finite(tid, sq[buf]) || Move::any_not_finite(tid, sd[buf]))) odd = 1;
+        __syncthreads();                             // tile `it` is there for all, and tile `it` - 1 is read
+        if (DIRECT) send(it + STAGES - 1, (it + STAGES - 1) % STAGES);
+        step(j0, sq[buf], sd[buf], ss[buf]);
+        if (!DIRECT) __syncthreads();                // a copy fills the tile that was just used STAGES turns before
+    }
+    if (DIRECT) arrived();
     if (!mine) return;
+    if (first && key < A.mask.sinks) {
+        float *pk = part_of(A, extra ? chunk_slot(A, s, packed, s.tile) : s.b, kv) + key * A.dim, *pv = pk + A.mask.sinks * A.dim;
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int e = d * 32 + row_of(r) + 4 * h;
+                if (e < A.dim) {
+                    pk[e] = dk[d][r];
+                    pv[e] = dv[d][r];
+                }
+            }
+        return;
+    }
     T *kd = seq_base<T>(A.dk, s, s.k0, packed, kv) + key * A.dk.row, *vd = seq_base<T>(A.dv, s, s.k0, packed, kv) + key * A.dv.row;
 #pragma unroll
     for (int d = 0; d < ND; ++d)
@@ -287,12 +356,66 @@ __global__ __launch_bounds__(256, 1) void grad_kv_kernel(WindowArgs A) {
         }
 }
 
-struct GradKernels { const void *delta, *q, *kv; };
-template <typename T> static GradKernels grads_of(int dim) {
-    const void *d = (const void *)delta_kernel<T>;
-    if (dim <= 64) return {d, (const void *)grad_q_kernel<T, 64>, (const void *)grad_kv_kernel<T, 64>};
-    if (dim <= 96) return {d, (const void *)grad_q_kernel<T, 96>, (const void *)grad_kv_kernel<T, 96>};
-    return {d, (const void *)grad_q_kernel<T, 128>, (const void *)grad_kv_kernel<T, 128>};
+// One wave a (sequence, key head, first key): the window's part and the chunks' parts, in order.
+template <typename T> __global__ __launch_bounds__(64) void join_kernel(WindowArgs A) {
+    const bool packed = A.cu_q != nullptr;
+    int id = (int)blockIdx.x;
+    const int key = id % A.mask.sinks; id /= A.mask.sinks;
+    const int kv = id % A.kv_heads, b = id / A.kv_heads;
+    Seq s;
+    s.b = b;
+    if (packed) {
+        auto at = [&](const int32_t *cu, int i, int64_t lo, int64_t hi) { return min(max((int64_t)cu[i], lo), hi); };
+        s.q0 = at(A.cu_q, b, 0, A.q_len);
+        s.k0 = at(A.cu_k, b, 0, A.k_len);
+        s.nq = (int)(at(A.cu_q, b + 1, s.q0, A.q_len) - s.q0);
+        s.nk = (int)(at(A.cu_k, b + 1, s.k0, A.k_len) - s.k0);
+    } else {
+        s.q0 = s.k0 = 0;
+        s.nq = (int)A.q_len;
+        s.nk = (int)A.k_len;
+    }
+    if (key >= s.nk) return;
+    const int end = window_end(A, s, min(GM, s.nk) - 1);
+    for (int e = threadIdx.x; e < 2 * A.dim; e += 64) {
+        const int64_t x = (int64_t)(e / A.dim * A.mask.sinks + key) * A.dim + e % A.dim;       // keys' gradients, then values'
+        float sum = part_of(A, b, kv)[x];
+        // the chunks that hold queries behind the window's last
+        for (int c = max(0, end + 1) / A.chunk; end + 1 < s.nq && c * (int64_t)A.chunk < s.nq; ++c)
+            sum += part_of(A, chunk_slot(A, s, packed, c), kv)[x];
+        const Rows &R = e < A.dim ? A.dk : A.dv;
+        seq_base<T>(R, s, s.k0, packed, kv)[key * R.row + e % A.dim] = narrow<T>(e < A.dim ? sum * A.scale : sum);
+    }
+}
+
+struct GradKernels { const void *delta, *q, *kv, *join; };
+template <typename T, int DP> static GradKernels grads_for(bool direct_q, bool direct_kv) {
+    return {(const void *)delta_kernel<T>,
+            direct_q ? (const void *)grad_q_kernel<T, DP, true> : (const void *)grad_q_kernel<T, DP, false>,
+            direct_kv ? (const void *)grad_kv_kernel<T, DP, true> : (const void *)grad_kv_kernel<T, DP, false>,
+            (const void *)join_kernel<T>};
+}
+template <typename T> static GradKernels grads_of(int dim, bool direct_q, bool direct_kv) {
+    return dim <= 64 ? grads_for<T, 64>(direct_q, direct_kv) : dim <= 96 ? grads_for<T, 96>(direct_q, direct_kv)
+                                                                        : grads_for<T, 128>(direct_q, direct_kv);
+}
+
+// Workspace: two floats a query row and head, then the first keys' parts where they are split.
+struct GradWork { int64_t stats, part, total; int chunk; };
+static int grad_work(const spmm_attn_desc_t *a, const char *where, bool packed, GradWork *w) {
+    const int64_t n = packed ? 1 : a->batch;
+    if (n && a->q_len > (INT64_C(1) << 44) / n / a->heads) return fail(SPMM_HIP_ERR_OVERFLOW, "%s: too many rows", where);
+    w->stats = (n * a->q_len * a->heads * 8 + 15) / 16 * 16;
+    w->chunk = 0;
+    w->part = 0;
+    const int64_t span = ((int64_t)a->window + GM + GN - 1) / GN * GN;      // queries of an ordinary block
+    if (a->window > 0 && a->window < a->k_len && a->sinks > 0 && a->sinks <= GM && a->k_len > a->sinks && a->q_len > 2 * span) {
+        w->chunk = (int)(span < 512 ? 512 : span);
+        const int64_t slots = a->batch + (packed ? a->q_len / w->chunk + a->batch : a->batch * ((a->q_len + w->chunk - 1) / w->chunk));
+        w->part = slots * a->kv_heads * 2 * a->sinks * a->dim * 4;
+    }
+    w->total = w->stats + w->part;
+    return SPMM_HIP_OK;
 }
 
 }  // namespace attn
@@ -303,10 +426,10 @@ extern "C" int spmm_attn_window_work(const spmm_attn_desc_t *a, int32_t packed, 
     const int st = check_desc(a, "attn_window_work");
     if (st != SPMM_HIP_OK) return st;
     if (!bytes) return fail(SPMM_HIP_ERR_ARG, "attn_window_work: bytes is NULL");
-    const int64_t n = packed ? 1 : a->batch;
-    if (n && a->q_len > (INT64_C(1) << 44) / n / a->heads) return fail(SPMM_HIP_ERR_OVERFLOW, "attn_window_work: too many rows");
-    *bytes = (size_t)(n * a->q_len * a->heads) * 4;
-    return SPMM_HIP_OK;
+    GradWork w;
+    const int sw = grad_work(a, "attn_window_work", packed != 0, &w);
+    if (sw == SPMM_HIP_OK) *bytes = (size_t)w.total;
+    return sw;
 }
 
 extern "C" int spmm_attn_window_grad(const spmm_attn_desc_t *a, const spmm_attn_rows_t *dout, const spmm_attn_rows_t *q,
@@ -331,27 +454,33 @@ extern "C" int spmm_attn_window_grad(const spmm_attn_desc_t *a, const spmm_attn_
         (st = check_rows(a, dv, W, "dv", nb, a->k_len, a->kv_heads, true, &A.dv)))
         return st;
     if (a->batch == 0) return SPMM_HIP_OK;
-    size_t need = 0;
-    if ((st = spmm_attn_window_work(a, packed, &need))) return st;
-    if (need > 0) {
-        if (!lse || (uintptr_t)lse % 4) return fail(SPMM_HIP_ERR_ARG, "%s: lse is NULL or not aligned", W);
-        if (!work || (uintptr_t)work % 16 || work_bytes < need)
-            return fail(SPMM_HIP_ERR_ARG, "%s: the workspace needs %zu bytes, 16-byte aligned", W, need);
+    GradWork w;
+    if ((st = grad_work(a, W, packed, &w))) return st;
+    if (w.total > 0) {
+        if (a->q_len > 0 && (!lse || (uintptr_t)lse % 4)) return fail(SPMM_HIP_ERR_ARG, "%s: lse is NULL or not aligned", W);
+        if (!work || (uintptr_t)work % 16 || work_bytes < (size_t)w.total)
+            return fail(SPMM_HIP_ERR_ARG, "%s: the workspace needs %lld bytes, 16-byte aligned", W, (long long)w.total);
     }
     A.lse = const_cast<float *>(lse);
-    A.delta = (float *)work;
-    int qt = 0, kt = 0;
+    A.stats = (float *)work;
+    A.part = (float *)((char *)work + w.stats);
+    A.chunk = w.chunk;
+    int qt = 0, kt = 0, ct = 0;
     if (a->q_len > 0 && (st = tile_count(a, W, packed, a->q_len, GM, &qt))) return st;
     if (a->k_len > 0 && (st = tile_count(a, W, packed, a->k_len, GM, &kt))) return st;
+    if (w.chunk && (st = tile_count(a, W, packed, a->q_len, w.chunk, &ct))) return st;
     OnDevice on(a->device, W);
     if (on.status) return on.status;
-    const GradKernels G = a->dtype == SPMM_ATTN_F32 ? grads_of<float>(a->dim)
-                          : a->dtype == SPMM_ATTN_F16 ? grads_of<_Float16>(a->dim) : grads_of<__bf16>(a->dim);
+    const bool dq_direct = A.k.direct && A.v.direct, dkv_direct = A.q.direct && A.dout.direct;
+    const GradKernels G = a->dtype == SPMM_ATTN_F32 ? grads_of<float>(a->dim, dq_direct, dkv_direct)
+                          : a->dtype == SPMM_ATTN_F16 ? grads_of<_Float16>(a->dim, dq_direct, dkv_direct)
+                                                      : grads_of<__bf16>(a->dim, dq_direct, dkv_direct);
     void *args[] = {&A};
     const int64_t rows = nb * a->q_len * a->heads;
     if ((st = launch(G.delta, W, (rows + 15) / 16, 256, args, stream))) return st;
     A.tiles = kt;
-    if ((st = launch(G.kv, W, (int64_t)kt * a->kv_heads, 256, args, stream))) return st;
+    if ((st = launch(G.kv, W, ((int64_t)kt + ct) * a->kv_heads, 256, args, stream))) return st;
+    if (w.chunk && (st = launch(G.join, W, a->batch * a->kv_heads * A.mask.sinks, 64, args, stream))) return st;
     A.tiles = qt;
     return launch(G.q, W, (int64_t)qt * a->heads, 256, args, stream);
 }

@@ -133,13 +133,13 @@ def test_bad_window_operands(A):
         assert grad(A, dk=rows(A, **bad)) == -1 and grad(A, dv=rows(A, **bad)) == -1
     for name in ("dout", "q", "k", "v", "out", "dq", "dk", "dv"):
         assert grad(A, **{name: None}) == -1 and grad(A, **{name: rows(A, ptr=None)}) == -1
-    assert grad(A, work=None) == -1 and grad(A, work=P + 8) == -1 and grad(A, nbytes=2 * 16 * 4 * 4 - 1) == -1
+    assert grad(A, work=None) == -1 and grad(A, work=P + 8) == -1 and grad(A, nbytes=2 * 16 * 4 * 8 - 1) == -1
 
 
 def test_workspaces(A):
     n = C.c_size_t()
-    assert A.lib.spmm_attn_window_work(desc(A, batch=3, q_len=7, heads=4), 0, n) == 0 and n.value == 3 * 7 * 4 * 4
-    assert A.lib.spmm_attn_window_work(desc(A, batch=3, q_len=7, heads=4), 1, n) == 0 and n.value == 7 * 4 * 4
+    assert A.lib.spmm_attn_window_work(desc(A, batch=3, q_len=7, heads=4), 0, n) == 0 and n.value == 3 * 7 * 4 * 8
+    assert A.lib.spmm_attn_window_work(desc(A, batch=3, q_len=7, heads=4), 1, n) == 0 and n.value == 7 * 4 * 8
     assert A.lib.spmm_attn_window_work(desc(A, batch=2 ** 29, q_len=2 ** 29), 0, n) == -7
     assert A.lib.spmm_attn_paged_work(desc(A), -1, n) == -1 and A.lib.spmm_attn_paged_work(desc(A), 2 ** 31, n) == -1
     assert A.lib.spmm_attn_paged_work(desc(A, window=0), 10, n) == 0 and n.value == 0     # one part: nothing to join
