@@ -7,6 +7,7 @@
 #include <cstdarg>
 #include <cstdint>
 #include <cstdio>
+#include <type_traits>
 
 #include "../../include/spmm_attn.h"
 
@@ -123,8 +124,6 @@ template <typename T, int DP> struct Tile {
     }
 };
 
-typedef __attribute__((address_space(3))) void lds_void;
-
 // Buffer loads that write LDS: lane l fills the l-th 16 (or 4) bytes from `tile` on with those at byte `off` of the buffer,
 // zeros where that lies outside.  The compiler does not count these loads: LDS is read after arrived<n>() (all of this
 // wave's but the last n are there) and a barrier, and a wave has waited for all before it ends.  (With the builtin
@@ -138,7 +137,8 @@ struct Buffer {
         const uint64_t b = (uint64_t)base;
         rsrc = i32x4{uniform((int)b), uniform((int)(b >> 32)) & 0xffff, uniform(bytes), 0x00027000};
     }
-    static __device__ __forceinline__ int place(const void *tile) { return uniform((int)(uintptr_t)(lds_void *)tile); }
+    // where in LDS: the low half of the address
+    static __device__ __forceinline__ int place(const void *tile) { return uniform((int)(uint32_t)(uintptr_t)tile); }
     __device__ __forceinline__ void to_lds16(void *tile, int off) const {
         asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(place(tile)), "v"(off), "s"(rsrc) : "memory");
     }

@@ -87,10 +87,8 @@ __global__ __launch_bounds__(256, 2) void window_kernel(WindowArgs A) {
     };
 
     f32x16 o[ND];
-#pragma unroll
-    for (int d = 0; d < ND; ++d) o[d] = zero16();
-    float m = -INFINITY, sum = 0.f;                  // of the scores times scale2
-    auto step = [&](int j0, const T *tk, const T *tv) {
+    float m, sum;                                    // of the scores times scale2
+    auto step = [&](auto careful, int j0, const T *tk, const T *tv) {
         if (w0 > w1 || !A.mask.any(w0, w1, j0, j0 + BN - 1)) return;
         const bool full = A.mask.all(w0, w1, j0, j0 + BN - 1);
         f32x16 sc[NK];
@@ -102,6 +100,7 @@ __global__ __launch_bounds__(256, 2) void window_kernel(WindowArgs A) {
                 sc[n] = mma32(L::row_frag(tk, n * 32 + (lane & 31), st * 16 + h * 8), qf[st], sc[n]);
         }
         if (!full) {
+            asm volatile("");                        // a branch, not 32 selects in every tile
 #pragma unroll
             for (int n = 0; n < NK; ++n)
 #pragma unroll
@@ -130,8 +129,7 @@ __global__ __launch_bounds__(256, 2) void window_kernel(WindowArgs A) {
                 sc[n][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[n][r], scale2, -base));
                 sum += sc[n][r];
             }
-        const bool careful = !full && __builtin_amdgcn_readfirstlane(odd);
-        if (!careful) {
+        if constexpr (!careful) {
 #pragma unroll
             for (int n = 0; n < NK; ++n)
 #pragma unroll
@@ -150,19 +148,32 @@ __global__ __launch_bounds__(256, 2) void window_kernel(WindowArgs A) {
         }
     };
 
-    __syncthreads();                                 // `odd` is set
-    if (tiles) {
-        if (DIRECT) send(tile_at(0), sk[0], sv[0]);
-        settle(tile_at(0), sk[0], sv[0]);
-    }
-    __syncthreads();
-    for (int it = 0; it < tiles; ++it) {             // a tile's loads are under way while the one before it is used
-        const int buf = it & 1;
-        const bool more = it + 1 < tiles;
-        if (DIRECT && more) send(tile_at(it + 1), sk[buf ^ 1], sv[buf ^ 1]);
-        step(tile_at(it), sk[buf], sv[buf]);
-        if (more) settle(tile_at(it + 1), sk[buf ^ 1], sv[buf ^ 1]);
+    // All tiles in turn; false if a value in a partly seen one is not finite and `careful` does not allow for that.
+    auto run = [&](auto careful) {
+        m = -INFINITY;
+        sum = 0.f;
+#pragma unroll
+        for (int d = 0; d < ND; ++d) o[d] = zero16();
+        if (tiles) {
+            if (DIRECT) send(tile_at(0), sk[0], sv[0]);
+            settle(tile_at(0), sk[0], sv[0]);
+        }
         __syncthreads();
+        for (int it = 0; it < tiles; ++it) {         // a tile's loads are under way while the one before it is used
+            const int buf = it & 1, j0 = tile_at(it);
+            if (!careful && !A.mask.all(pmin, pmax, j0, j0 + BN - 1) && uniform(odd)) return false;
+            const bool more = it + 1 < tiles;
+            if (DIRECT && more) send(tile_at(it + 1), sk[buf ^ 1], sv[buf ^ 1]);
+            step(careful, j0, sk[buf], sv[buf]);
+            if (more) settle(tile_at(it + 1), sk[buf ^ 1], sv[buf ^ 1]);
+            __syncthreads();
+        }
+        return true;
+    };
+    __syncthreads();                                 // `odd` is set
+    if (!run(std::false_type{})) {                   // the whole block leaves at the same tile
+        __syncthreads();
+        run(std::true_type{});
     }
     sum += __shfl_xor(sum, 32);
     if (!mine) return;

@@ -106,9 +106,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void grad_q_kernel(Win
         if (!A.mask.all(pmin, pmax, j0, j0 + GN - 1) && Move::any_not_finite(tid, tk)) odd = 1;
     };
     f32x16 dq[ND];
-#pragma unroll
-    for (int d = 0; d < ND; ++d) dq[d] = zero16();
-    auto step = [&](int j0, const T *tk, const T *tv) {
+    auto step = [&](auto careful, int j0, const T *tk, const T *tv) {
         if (w0 > w1 || !A.mask.any(w0, w1, j0, j0 + GN - 1)) return;
         const bool full = A.mask.all(w0, w1, j0, j0 + GN - 1);
         f32x16 sc = zero16(), dp = zero16();
@@ -121,13 +119,13 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void grad_q_kernel(Win
         for (int r = 0; r < 16; ++r)
             sc[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[r], A.scale2, -lse2)) * (dp[r] - delta);
         if (!full) {
+            asm volatile("");                        // a branch, not 16 selects in every tile
 #pragma unroll
             for (int r = 0; r < 16; ++r)
                 if (!A.mask.sees(p, j0 + row_of(r) + 4 * h)) sc[r] = 0.f;
         }
         // a seen key that is not finite makes the row's weights NaN, so it need not be put back
-        const bool careful = !full && uniform(odd);
-        if (!careful) {
+        if constexpr (!careful) {
 #pragma unroll
             for (int k2 = 0; k2 < 2; ++k2) {
                 const frag<T> dsf = next_operand<T>(sc, k2);
@@ -142,19 +140,30 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void grad_q_kernel(Win
             for (int d = 0; d < ND; ++d) dq[d] = c.acc[d];
         }
     };
-    __syncthreads();
-    if (tiles) {
-        if (DIRECT) send(tile_at(0), sk[0], sv[0]);
-        settle(tile_at(0), sk[0], sv[0]);
-    }
-    __syncthreads();
-    for (int it = 0; it < tiles; ++it) {
-        const int buf = it & 1;
-        const bool more = it + 1 < tiles;
-        if (DIRECT && more) send(tile_at(it + 1), sk[buf ^ 1], sv[buf ^ 1]);
-        step(tile_at(it), sk[buf], sv[buf]);
-        if (more) settle(tile_at(it + 1), sk[buf ^ 1], sv[buf ^ 1]);
+    // as in the forward kernel: false if a value in a partly seen tile is not finite
+    auto run = [&](auto careful) {
+#pragma unroll
+        for (int d = 0; d < ND; ++d) dq[d] = zero16();
+        if (tiles) {
+            if (DIRECT) send(tile_at(0), sk[0], sv[0]);
+            settle(tile_at(0), sk[0], sv[0]);
+        }
         __syncthreads();
+        for (int it = 0; it < tiles; ++it) {
+            const int buf = it & 1, j0 = tile_at(it);
+            if (!careful && !A.mask.all(pmin, pmax, j0, j0 + GN - 1) && uniform(odd)) return false;
+            const bool more = it + 1 < tiles;
+            if (DIRECT && more) send(tile_at(it + 1), sk[buf ^ 1], sv[buf ^ 1]);
+            step(careful, j0, sk[buf], sv[buf]);
+            if (more) settle(tile_at(it + 1), sk[buf ^ 1], sv[buf ^ 1]);
+            __syncthreads();
+        }
+        return true;
+    };
+    __syncthreads();
+    if (!run(std::false_type{})) {
+        __syncthreads();
+        run(std::true_type{});
     }
     if (!mine) return;
     T *dst = seq_base<T>(A.dq, s, s.q0, packed, head) + i * A.dq.row;
@@ -259,10 +268,8 @@ __global__ __launch_bounds__(256, 1) void grad_kv_kernel(WindowArgs A) {
         if (tid < 2 * GN) ss[buf][tid] = j0 + tid / 2 < s.nq ? stats[((int64_t)(j0 + tid / 2) * A.heads + head) * 2 + tid % 2] : 0.f;
     };
     f32x16 dk[ND], dv[ND];
-#pragma unroll
-    for (int d = 0; d < ND; ++d) dk[d] = dv[d] = zero16();
     // rows behind the last query are zeros, lse and D too: P = 1 then, and adds 1 * 0
-    auto step = [&](int j0, const T *tq, const T *td, const float *ts) {
+    auto step = [&](auto careful, int j0, const T *tq, const T *td, const float *ts) {
         const int p0 = j0 + shift;
         if (c0 > c1 || !A.mask.any(p0, p0 + GN - 1, c0, c1)) return;
         const bool full = A.mask.all(p0, p0 + GN - 1, c0, c1) && j0 >= i0 && j0 + GN - 1 <= i1;
@@ -282,14 +289,14 @@ __global__ __launch_bounds__(256, 1) void grad_kv_kernel(WindowArgs A) {
             }
         }
         if (!full) {
+            asm volatile("");
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
                 const int i = j0 + row_of(r) + 4 * h;
                 if (i < i0 || i > i1 || !A.mask.sees(i + shift, key)) sc[r] = dp[r] = 0.f;
             }
         }
-        const bool careful = !full && uniform(odd);
-        if (!careful) {
+        if constexpr (!careful) {
 #pragma unroll
             for (int k2 = 0; k2 < 2; ++k2) {
                 const frag<T> pf = next_operand<T>(sc, k2), dsf = next_operand<T>(dp, k2);
@@ -312,21 +319,32 @@ __global__ __launch_bounds__(256, 1) void grad_kv_kernel(WindowArgs A) {
             for (int d = 0; d < ND; ++d) dk[d] = c.acc[d];
         }
     };
-    __syncthreads();
-    if (DIRECT) {
+    auto run = [&](auto careful) {
 #pragma unroll
-        for (int it = 0; it < STAGES - 1; ++it) send(it, it);
-    }
-    for (int it = 0; it < tiles; ++it) {
-        const int buf = it % STAGES, j0 = (q0t + it % nqt) * GN, p0 = j0 + shift;
-        if (DIRECT) arrived<(STAGES - 2) * LOADS>();
-        else copy(it, buf);
-        if (!(A.mask.all(p0, p0 + GN - 1, n0, n1) && j0 >= i0 && j0 + GN - 1 <= i1) &&
-            (Move::any_not_finite(tid, sq[buf]) || Move::any_not_finite(tid, sd[buf]))) odd = 1;
-        __syncthreads();                             // tile `it` is there for all, and tile `it` - 1 is read
-        if (DIRECT) send(it + STAGES - 1, (it + STAGES - 1) % STAGES);
-        step(j0, sq[buf], sd[buf], ss[buf]);
-        if (!DIRECT) __syncthreads();                // a copy fills the tile that was just used STAGES turns before
+        for (int d = 0; d < ND; ++d) dk[d] = dv[d] = zero16();
+        if (DIRECT) {
+#pragma unroll
+            for (int it = 0; it < STAGES - 1; ++it) send(it, it);
+        }
+        for (int it = 0; it < tiles; ++it) {
+            const int buf = it % STAGES, j0 = (q0t + it % nqt) * GN, p0 = j0 + shift;
+            if (DIRECT) arrived<(STAGES - 2) * LOADS>();
+            else copy(it, buf);
+            const bool whole = A.mask.all(p0, p0 + GN - 1, n0, n1) && j0 >= i0 && j0 + GN - 1 <= i1;
+            if (!whole && (Move::any_not_finite(tid, sq[buf]) || Move::any_not_finite(tid, sd[buf]))) odd = 1;
+            __syncthreads();                         // tile `it` is there for all, and tile `it` - 1 is read
+            if (!careful && !whole && uniform(odd)) return false;
+            if (DIRECT) send(it + STAGES - 1, (it + STAGES - 1) % STAGES);
+            step(careful, j0, sq[buf], sd[buf], ss[buf]);
+            if (!DIRECT) __syncthreads();
+        }
+        return true;
+    };
+    __syncthreads();
+    if (!run(std::false_type{})) {
+        if (DIRECT) arrived();
+        __syncthreads();
+        run(std::true_type{});
     }
     if (DIRECT) arrived();
     if (!mine) return;
