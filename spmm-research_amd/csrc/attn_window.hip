@@ -11,6 +11,7 @@ namespace attn {
 
 template <typename T> constexpr int BN_OF = sizeof(T) == 2 ? 64 : 32;      // keys of a tile
 constexpr int BM = 128;                                                      // queries of a workgroup
+constexpr float SLACK = 8.f;
 
 template <typename T, int DP, bool DIRECT>
 __global__ __launch_bounds__(256, 2) void window_kernel(WindowArgs A) {
@@ -89,7 +90,8 @@ __global__ __launch_bounds__(256, 2) void window_kernel(WindowArgs A) {
     f32x16 o[ND];
     float m, sum;                                    // of the scores times scale2
     auto step = [&](auto careful, int j0, const T *tk, const T *tv) {
-        if (w0 > w1 || !A.mask.any(w0, w1, j0, j0 + BN - 1)) return;
+        // A wave whose queries see none of the block's tile goes through it all the same: a way round it would have the
+        // accumulators copied at the end of every turn.
         const bool full = A.mask.all(w0, w1, j0, j0 + BN - 1);
         f32x16 sc[NK];
 #pragma unroll
@@ -112,16 +114,20 @@ __global__ __launch_bounds__(256, 2) void window_kernel(WindowArgs A) {
         for (int n = 0; n < NK; ++n)
 #pragma unroll
             for (int r = 0; r < 16; ++r) mx = fmaxf(mx, sc[n][r]);
-        mx = fmaxf(mx, __shfl_xor(mx, 32));
-        mx = fmaxf(m, mx * scale2);
-        const float base = mx == -INFINITY ? 0.f : mx;
-        if (__any(mx != m)) {
-            const float alpha = __builtin_amdgcn_exp2f(m - base);
+        mx = fmaxf(mx, __shfl_xor(mx, 32)) * scale2;
+        // The exponentials' base follows the maximum only when that has grown by more than SLACK: weights up to
+        // 2^SLACK lose nothing in any of the types, and the accumulators are rarely rescaled.
+        // Each query by itself: its result then does not depend on which others share its wave.
+        const bool grown = mx > m + SLACK;
+        if (__any(grown)) {
+            const float top = grown ? mx : m;
+            const float alpha = grown ? __builtin_amdgcn_exp2f(m - top) : 1.f;
             sum *= alpha;
 #pragma unroll
             for (int d = 0; d < ND; ++d) o[d] *= alpha;
-            m = mx;
+            m = top;
         }
+        const float base = m == -INFINITY ? 0.f : m;
 #pragma unroll
         for (int n = 0; n < NK; ++n)
 #pragma unroll
