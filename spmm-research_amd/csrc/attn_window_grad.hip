@@ -107,7 +107,6 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void grad_q_kernel(Win
     };
     f32x16 dq[ND];
     auto step = [&](auto careful, int j0, const T *tk, const T *tv) {
-        if (w0 > w1 || !A.mask.any(w0, w1, j0, j0 + GN - 1)) return;
         const bool full = A.mask.all(w0, w1, j0, j0 + GN - 1);
         f32x16 sc = zero16(), dp = zero16();
 #pragma unroll
@@ -192,13 +191,21 @@ __device__ __forceinline__ int window_end(const WindowArgs &A, const Seq &s, int
 
 constexpr int STAGES = 4;                    // tiles of queries on their way or in use
 
-template <typename T, int DP, bool DIRECT>
-__global__ __launch_bounds__(256, 1) void grad_kv_kernel(WindowArgs A) {
+template <typename T, int DP> struct KvShared {
+    __align__(16) T q[STAGES][GN * Tile<T, DP>::PITCH], d[STAGES][GN * Tile<T, DP>::PITCH];
+    __align__(16) float s[STAGES][2 * GN];                           // lse and D of the tile's rows
+    int odd;
+};
+
+// False, with nothing written, if a value in a partly seen tile is not finite and CAREFUL does not allow for that.
+template <typename T, int DP, bool DIRECT, bool CAREFUL>
+__device__ __forceinline__ bool grad_kv_block(const WindowArgs &A, KvShared<T, DP> &sh) {
     using L = Tile<T, DP>;
     constexpr int ND = DP / 32, NS = DP / 16;
-    __shared__ __align__(16) T sq[STAGES][GN * L::PITCH], sd[STAGES][GN * L::PITCH];
-    __shared__ __align__(16) float ss[STAGES][2 * GN];              // lse and D of the tile's rows
-    __shared__ int odd;
+    auto &sq = sh.q;
+    auto &sd = sh.d;
+    auto &ss = sh.s;
+    int &odd = sh.odd;
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), h = lane >> 5;
     int kv, g, t;
     place(A, 1, &kv, &g, &t);
@@ -212,7 +219,7 @@ __global__ __launch_bounds__(256, 1) void grad_kv_kernel(WindowArgs A) {
             zero_rows<T>(A.dk, from, step, GM, A.k_len, kv, A.dim);
             zero_rows<T>(A.dv, from, step, GM, A.k_len, kv, A.dim);
         }
-        return;
+        return true;
     }
     if (tid == 0) odd = 0;
     const int group = A.heads / A.kv_heads;
@@ -225,7 +232,7 @@ __global__ __launch_bounds__(256, 1) void grad_kv_kernel(WindowArgs A) {
     if (extra) {
         i0 = max(s.tile * A.chunk, window_end(A, s, min(GM, s.nk) - 1) + 1);
         i1 = min((s.tile + 1) * A.chunk, s.nq) - 1;
-        if (i1 < i0 || n1 < 0) return;
+        if (i1 < i0 || n1 < 0) return true;
     }
     const int q0t = i0 / GN, nqt = i1 >= i0 ? i1 / GN - q0t + 1 : 0, tiles = nqt * group;
 
@@ -268,42 +275,62 @@ __global__ __launch_bounds__(256, 1) void grad_kv_kernel(WindowArgs A) {
         if (tid < 2 * GN) ss[buf][tid] = j0 + tid / 2 < s.nq ? stats[((int64_t)(j0 + tid / 2) * A.heads + head) * 2 + tid % 2] : 0.f;
     };
     f32x16 dk[ND], dv[ND];
+    // the positions plo .. plo + seen - 1 are those of the block's queries that see this lane's key
+    const int plo = max(key, i0 + shift);
+    const int phi = min(i1 + shift, A.mask.window == 0 || key < A.mask.sinks ? INT32_MAX : key + A.mask.window - 1);
+    const unsigned seen = (unsigned)max(0, phi - plo + 1);
     // rows behind the last query are zeros, lse and D too: P = 1 then, and adds 1 * 0
-    auto step = [&](auto careful, int j0, const T *tq, const T *td, const float *ts) {
+    auto step = [&](int j0, const T *tq, const T *td, const float *ts) {
         const int p0 = j0 + shift;
-        if (c0 > c1 || !A.mask.any(p0, p0 + GN - 1, c0, c1)) return;
         const bool full = A.mask.all(p0, p0 + GN - 1, c0, c1) && j0 >= i0 && j0 + GN - 1 <= i1;
+        // Every read from LDS is issued well before its product: the only wave of a SIMD has none to hide behind.
+        frag<T> ra[NS], rb[NS];
+#pragma unroll
+        for (int st = 0; st < NS; ++st) {
+            ra[st] = L::row_frag(tq, lane & 31, st * 16 + h * 8);
+            rb[st] = L::row_frag(td, lane & 31, st * 16 + h * 8);
+        }
+        f32x4 stat[8];
+#pragma unroll
+        for (int r = 0; r < 8; ++r) stat[r] = *reinterpret_cast<const f32x4 *>(ts + 2 * (row_of(2 * r) + 4 * h));
+        __builtin_amdgcn_sched_barrier(0);
         f32x16 sc = zero16(), dp = zero16();
 #pragma unroll
         for (int st = 0; st < NS; ++st) {
-            sc = mma32(L::row_frag(tq, lane & 31, st * 16 + h * 8), kf[st], sc);
-            dp = mma32(L::row_frag(td, lane & 31, st * 16 + h * 8), vf[st], dp);
+            sc = mma32(ra[st], kf[st], sc);
+            dp = mma32(rb[st], vf[st], dp);
         }
+        __builtin_amdgcn_sched_barrier(0);
+        frag<T> co[2][ND], cq[2][ND];
+        if constexpr (!CAREFUL) {
 #pragma unroll
-        for (int r2 = 0; r2 < 16; r2 += 2) {
-            const f32x4 st = *reinterpret_cast<const f32x4 *>(ts + 2 * (row_of(r2) + 4 * h));
+            for (int k2 = 0; k2 < 2; ++k2)
 #pragma unroll
-            for (int r = r2; r < r2 + 2; ++r) {
-                sc[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[r], A.scale2, -st[2 * (r - r2)]));
-                dp[r] = sc[r] * (dp[r] - st[2 * (r - r2) + 1]);
-            }
+                for (int d = 0; d < ND; ++d) {
+                    co[k2][d] = L::col_frag(td, k2 * 16, d * 32, lane);
+                    cq[k2][d] = L::col_frag(tq, k2 * 16, d * 32, lane);
+                }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            sc[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[r], A.scale2, -stat[r / 2][2 * (r % 2)]));
+            dp[r] = sc[r] * (dp[r] - stat[r / 2][2 * (r % 2) + 1]);
         }
         if (!full) {
             asm volatile("");
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int i = j0 + row_of(r) + 4 * h;
-                if (i < i0 || i > i1 || !A.mask.sees(i + shift, key)) sc[r] = dp[r] = 0.f;
-            }
+            for (int r = 0; r < 16; ++r)
+                if ((unsigned)(p0 + row_of(r) + 4 * h - plo) >= seen) sc[r] = dp[r] = 0.f;
         }
-        if constexpr (!careful) {
+        if constexpr (!CAREFUL) {
 #pragma unroll
             for (int k2 = 0; k2 < 2; ++k2) {
                 const frag<T> pf = next_operand<T>(sc, k2), dsf = next_operand<T>(dp, k2);
 #pragma unroll
                 for (int d = 0; d < ND; ++d) {
-                    dv[d] = mma32(L::col_frag(td, k2 * 16, d * 32, lane), pf, dv[d]);
-                    dk[d] = mma32(L::col_frag(tq, k2 * 16, d * 32, lane), dsf, dk[d]);
+                    dv[d] = mma32(co[k2][d], pf, dv[d]);
+                    dk[d] = mma32(cq[k2][d], dsf, dk[d]);
                 }
             }
         } else {
@@ -319,35 +346,32 @@ __global__ __launch_bounds__(256, 1) void grad_kv_kernel(WindowArgs A) {
             for (int d = 0; d < ND; ++d) dk[d] = c.acc[d];
         }
     };
-    auto run = [&](auto careful) {
 #pragma unroll
-        for (int d = 0; d < ND; ++d) dk[d] = dv[d] = zero16();
-        if (DIRECT) {
-#pragma unroll
-            for (int it = 0; it < STAGES - 1; ++it) send(it, it);
-        }
-        for (int it = 0; it < tiles; ++it) {
-            const int buf = it % STAGES, j0 = (q0t + it % nqt) * GN, p0 = j0 + shift;
-            if (DIRECT) arrived<(STAGES - 2) * LOADS>();
-            else copy(it, buf);
-            const bool whole = A.mask.all(p0, p0 + GN - 1, n0, n1) && j0 >= i0 && j0 + GN - 1 <= i1;
-            if (!whole && (Move::any_not_finite(tid, sq[buf]) || Move::any_not_finite(tid, sd[buf]))) odd = 1;
-            __syncthreads();                         // tile `it` is there for all, and tile `it` - 1 is read
-            if (!careful && !whole && uniform(odd)) return false;
-            if (DIRECT) send(it + STAGES - 1, (it + STAGES - 1) % STAGES);
-            step(careful, j0, sq[buf], sd[buf], ss[buf]);
-            if (!DIRECT) __syncthreads();
-        }
-        return true;
-    };
+    for (int d = 0; d < ND; ++d) dk[d] = dv[d] = zero16();
     __syncthreads();
-    if (!run(std::false_type{})) {
-        if (DIRECT) arrived();
-        __syncthreads();
-        run(std::true_type{});
+    if (DIRECT) {
+#pragma unroll
+        for (int it = 0; it < STAGES - 1; ++it) send(it, it);
+    }
+    bool fine = true;
+    for (int it = 0; it < tiles; ++it) {
+        const int buf = it % STAGES, j0 = (q0t + it % nqt) * GN, p0 = j0 + shift;
+        if (DIRECT) arrived<(STAGES - 2) * LOADS>();
+        else copy(it, buf);
+        const bool whole = A.mask.all(p0, p0 + GN - 1, n0, n1) && j0 >= i0 && j0 + GN - 1 <= i1;
+        if (!whole && (Move::any_not_finite(tid, sq[buf]) || Move::any_not_finite(tid, sd[buf]))) odd = 1;
+        __syncthreads();                             // tile `it` is there for all, and tile `it` - 1 is read
+        if (!CAREFUL && !whole && uniform(odd)) {    // the whole block leaves at the same tile
+            fine = false;
+            break;
+        }
+        if (DIRECT) send(it + STAGES - 1, (it + STAGES - 1) % STAGES);
+        step(j0, sq[buf], sd[buf], ss[buf]);
+        if (!DIRECT) __syncthreads();
     }
     if (DIRECT) arrived();
-    if (!mine) return;
+    if (!fine) return false;
+    if (!mine) return true;
     if (first && key < A.mask.sinks) {
         float *pk = part_of(A, extra ? chunk_slot(A, s, packed, s.tile) : s.b, kv) + key * A.dim, *pv = pk + A.mask.sinks * A.dim;
 #pragma unroll
@@ -360,7 +384,7 @@ __global__ __launch_bounds__(256, 1) void grad_kv_kernel(WindowArgs A) {
                     pv[e] = dv[d][r];
                 }
             }
-        return;
+        return true;
     }
     T *kd = seq_base<T>(A.dk, s, s.k0, packed, kv) + key * A.dk.row, *vd = seq_base<T>(A.dv, s, s.k0, packed, kv) + key * A.dv.row;
 #pragma unroll
@@ -372,6 +396,20 @@ __global__ __launch_bounds__(256, 1) void grad_kv_kernel(WindowArgs A) {
             store4<T>(vd, d * 32 + row_of(r) + 4 * h, A.dim, A.dv.wide,
                       f32x4{dv[d][r], dv[d][r + 1], dv[d][r + 2], dv[d][r + 3]});
         }
+    return true;
+}
+// The rare case in a function of its own, which takes no registers from the loop above.
+template <typename T, int DP>
+__device__ __attribute__((noinline)) void grad_kv_again(const WindowArgs *A, KvShared<T, DP> *sh) {
+    grad_kv_block<T, DP, false, true>(*A, *sh);
+}
+template <typename T, int DP, bool DIRECT> __global__ __launch_bounds__(256, 1) void grad_kv_kernel(WindowArgs A) {
+    __shared__ KvShared<T, DP> sh;
+    if (!grad_kv_block<T, DP, DIRECT, false>(A, sh)) {
+        __syncthreads();
+        const WindowArgs copy = A;
+        grad_kv_again<T, DP>(&copy, &sh);
+    }
 }
 
 // One wave a (sequence, key head, first key): the window's part and the chunks' parts, in order.
