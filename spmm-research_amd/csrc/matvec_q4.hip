@@ -68,93 +68,122 @@ struct Args {
     bool wide;
 };
 
-// 8 elements of part `part` of x[tok][k ...]
-template <typename T> __device__ __forceinline__ frag<typename Kind<T>::M> load_x(const Args &A, int64_t tok, int part, int64_t k, bool mine) {
-    using M = typename Kind<T>::M;
-    frag<M> f = {};
+// x[tok][k .. k + 7] as it stands in memory, zeros where there is none
+template <typename T> __device__ __forceinline__ frag<T> fetch_x(const Args &A, int64_t tok, int64_t k, bool mine) {
+    frag<T> f = {};
     if (!mine || k >= A.cols) return f;
     const T *p = (const T *)A.x + tok * A.x_stride + k;
-    T e[8];
     if (A.wide && k + 8 <= A.cols) {
-        __builtin_memcpy(e, __builtin_assume_aligned(p, 16), sizeof e);
+        __builtin_memcpy(&f, __builtin_assume_aligned(p, 16), sizeof f);
     } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) e[j] = k + j < A.cols ? p[j] : (T)0.f;
+        for (int j = 0; j < 8; ++j)
+            if (k + j < A.cols) f[j] = p[j];
     }
+    return f;
+}
+// Part `part` of it as an operand
+template <typename T> __device__ __forceinline__ frag<typename Kind<T>::M> part_x(const frag<T> &x, int part) {
+    if constexpr (sizeof(T) == 2) {
+        return x;
+    } else {
+        frag<__bf16> f;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        if constexpr (sizeof(T) == 2) {
-            f[j] = e[j];
-        } else {
+        for (int j = 0; j < 8; ++j) {
             // 8 bits of the value at a time, cut off, so each rest is exact; an infinity or NaN is all in the first part
-            float r = e[j];
+            float r = x[j];
             uint32_t hi = __builtin_bit_cast(uint32_t, r) & 0xffff0000u;
-            for (int i = 0; i < part; ++i) {
-                r = (hi & 0x7f800000u) == 0x7f800000u ? 0.f : r - __builtin_bit_cast(float, hi);
-                hi = __builtin_bit_cast(uint32_t, r) & 0xffff0000u;
+#pragma unroll
+            for (int i = 1; i <= 2; ++i) {
+                const float rest = (hi & 0x7f800000u) == 0x7f800000u ? 0.f : r - __builtin_bit_cast(float, hi);
+                if (part >= i) {
+                    r = rest;
+                    hi = __builtin_bit_cast(uint32_t, r) & 0xffff0000u;
+                }
             }
             if (part == 0 && r != r) hi |= 0x00400000u;
             f[j] = __builtin_bit_cast(__bf16, (uint16_t)(hi >> 16));
         }
+        return f;
     }
-    return f;
 }
 
-template <typename T, bool ZEROS> __global__ void matvec_kernel(Args A) {
+// A block takes RT row tiles, its waves share out the column tiles; SG scales a column tile.
+template <typename T, bool ZEROS, int RT, int SG> __global__ __launch_bounds__(WMAX * 64) void matvec_kernel(Args A) {
     using K = Kind<T>;
     using M = typename K::M;
     constexpr int PARTS = K::PARTS, PER = 16 / PARTS;        // vectors a block takes
+    typedef T t4 __attribute__((ext_vector_type(4)));
     __shared__ float part[WMAX][TR][17];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6, n = lane & 15, g4 = lane >> 4;
-    const int rt = blockIdx.x;
+    const int rt0 = blockIdx.x * RT;
     const int64_t t0 = (int64_t)blockIdx.y * PER, tok = t0 + n / PARTS;
     const bool mine = n < PER * PARTS && tok < A.tokens;
-    const uint4 *w = A.w + (int64_t)rt * A.tiles * 64 + lane;
     frag<M> one;
 #pragma unroll
     for (int j = 0; j < 8; ++j) one[j] = (M)1.f;
 
-    f32x4 y = {0.f, 0.f, 0.f, 0.f};
-    const int steps = A.group < TC ? A.group / 32 : 4;       // products of a scale
-    uint4 next = wave < A.tiles ? w[(int64_t)wave * 64] : make_uint4(0, 0, 0, 0);
+    f32x4 y[RT];
+#pragma unroll
+    for (int i = 0; i < RT; ++i) y[i] = f32x4{0.f, 0.f, 0.f, 0.f};
     for (int t = wave; t < A.tiles; t += waves) {
-        const uint4 now = next;
-        if (t + waves < A.tiles) next = w[(int64_t)(t + waves) * 64];
-        const uint32_t word[4] = {now.x, now.y, now.z, now.w};
-        f32x4 c = {0.f, 0.f, 0.f, 0.f}, sx = {0.f, 0.f, 0.f, 0.f};
+        // everything of the tile is asked for before anything is used; past the last row tile the last one again
+        uint4 w[RT];
+        t4 sc[RT][SG];
+        uint32_t z[RT][SG];
+        frag<T> xr[4];
+#pragma unroll
+        for (int i = 0; i < RT; ++i) w[i] = A.w[((int64_t)min(rt0 + i, A.row_tiles - 1) * A.tiles + t) * 64 + lane];
+#pragma unroll
+        for (int s = 0; s < 4; ++s) xr[s] = fetch_x<T>(A, tok, (int64_t)t * TC + s * 32 + g4 * 8, mine);
+#pragma unroll
+        for (int i = 0; i < RT; ++i)
+#pragma unroll
+            for (int g = 0; g < SG; ++g) {
+                const int gi = min((t * TC + g * (TC / SG)) / A.group, A.groups - 1);     // past the last column x is 0
+                const int64_t at = ((int64_t)min(rt0 + i, A.row_tiles - 1) * A.groups + gi) * TR + g4 * 4;
+                sc[i][g] = *(const t4 *)((const T *)A.scales + at);
+                z[i][g] = ZEROS ? A.zeros[at / 4] : 0x08080808u;
+            }
+        f32x4 c[RT], sx = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < RT; ++i) c[i] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
-            const int64_t k = (int64_t)t * TC + s * 32;
-            const frag<M> xf = load_x<T>(A, tok, n % PARTS, k + g4 * 8, mine);
-            c = mma(unpack<T>(word[s]), xf, c);
+            const frag<M> xf = part_x<T>(xr[s], n % PARTS);
             sx = mma(one, xf, sx);
-            if ((s + 1) % steps == 0) {
-                const int64_t gi = k / A.group;
-                if (gi < A.groups) {
-                    const int64_t at = ((int64_t)rt * A.groups + gi) * TR + g4 * 4;
-                    typedef T t4 __attribute__((ext_vector_type(4)));
-                    const t4 sc = *(const t4 *)((const T *)A.scales + at);
-                    const uint32_t z4 = ZEROS ? A.zeros[at / 4] : 0x08080808u;
+#pragma unroll
+            for (int i = 0; i < RT; ++i) c[i] = mma(unpack<T>(s == 0 ? w[i].x : s == 1 ? w[i].y : s == 2 ? w[i].z : w[i].w), xf, c[i]);
+            if ((s + 1) % (4 / SG) == 0) {
+                const int g = s / (4 / SG);
+#pragma unroll
+                for (int i = 0; i < RT; ++i) {
 #pragma unroll
                     for (int r = 0; r < 4; ++r)
-                        y[r] += (float)sc[r] * (c[r] - (float)(16 + ((z4 >> (8 * r)) & 255)) * sx[r]);
+                        y[i][r] += (float)sc[i][g][r] * (c[i][r] - (float)(16 + ((z[i][g] >> (8 * r)) & 255)) * sx[r]);
+                    c[i] = f32x4{0.f, 0.f, 0.f, 0.f};
                 }
-                c = sx = f32x4{0.f, 0.f, 0.f, 0.f};
+                sx = f32x4{0.f, 0.f, 0.f, 0.f};
             }
         }
     }
+    // the waves' sums in wave order, a row tile at a time
 #pragma unroll
-    for (int r = 0; r < 4; ++r) part[wave][g4 * 4 + r][n] = y[r];
-    __syncthreads();
-    for (int i = threadIdx.x; i < TR * PER; i += blockDim.x) {
-        const int r = i % TR, t = i / TR;
-        const int64_t row = (int64_t)rt * TR + r;
-        if (row >= A.rows || t0 + t >= A.tokens) continue;
-        float sum = 0.f;
-        for (int wv = 0; wv < waves; ++wv)
+    for (int i = 0; i < RT; ++i) {
+        if (i) __syncthreads();
 #pragma unroll
-            for (int p = 0; p < PARTS; ++p) sum += part[wv][r][t * PARTS + p];
-        ((T *)A.y)[(t0 + t) * A.y_stride + row] = (T)sum;
+        for (int r = 0; r < 4; ++r) part[wave][g4 * 4 + r][n] = y[i][r];
+        __syncthreads();
+        for (int e = threadIdx.x; e < TR * PER; e += blockDim.x) {
+            const int r = e % TR, t = e / TR;
+            const int64_t row = (int64_t)(rt0 + i) * TR + r;
+            if (row >= A.rows || t0 + t >= A.tokens) continue;
+            float sum = 0.f;
+            for (int wv = 0; wv < waves; ++wv)
+#pragma unroll
+                for (int p = 0; p < PARTS; ++p) sum += part[wv][r][t * PARTS + p];
+            ((T *)A.y)[(t0 + t) * A.y_stride + row] = (T)sum;
+        }
     }
 }
 
@@ -166,23 +195,41 @@ struct LayoutArgs {
     uint8_t *lz;
     int64_t rows, cols, packed_stride, scale_stride, zero_stride, words, entries;
     int tiles, groups;
+    bool words_aligned;
 };
+
+// Nibble j of 8 to place j / 2 + 4 (j % 2): the even ones to the low half, the odd ones to the high half.
+__device__ __forceinline__ uint32_t pair_up(uint32_t x) {
+    auto low = [](uint32_t v) {
+        v &= 0x0f0f0f0fu;
+        v = (v | v >> 4) & 0x00ff00ffu;
+        return (v | v >> 8) & 0xffffu;
+    };
+    return low(x) | low(x >> 4) << 16;
+}
 
 template <typename T> __global__ __launch_bounds__(256) void layout_kernel(LayoutArgs A) {
     const int64_t step = (int64_t)gridDim.x * blockDim.x, i0 = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-    for (int64_t i = i0; i < A.words; i += step) {
+    for (int64_t i = i0; i < A.words / 4; i += step) {
         // word s of lane l of tile (rt, t): row l % 16, columns 128 t + 32 s + 8 (l / 16) + 0..7
-        const int s = (int)(i & 3), l = (int)((i >> 2) & 63);
-        const int64_t tile = i >> 8, rt = tile / A.tiles, t = tile % A.tiles, row = rt * TR + (l & 15);
-        const int64_t c0 = t * TC + s * 32 + (l >> 4) * 8;
-        uint32_t out = 0;
-        for (int j = 0; j < 8; ++j) {
-            const int64_t c = c0 + j;
+        const int l = (int)(i & 63);
+        const int64_t tile = i >> 6, rt = tile / A.tiles, t = tile - rt * A.tiles, row = rt * TR + (l & 15);
+        uint32_t out[4];
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            const int64_t c = t * TC + s * 32 + (l >> 4) * 8;
             uint32_t q = 0;
-            if (row < A.rows && c < A.cols) q = (A.packed[row * A.packed_stride + c / 2] >> (4 * (c & 1))) & 15u;
-            out |= q << (4 * ((j >> 1) + 4 * (j & 1)));
+            if (row < A.rows && c < A.cols) {
+                const uint8_t *p = A.packed + row * A.packed_stride + c / 2;
+                if (A.words_aligned && c + 8 <= A.cols) {
+                    q = *(const uint32_t *)p;
+                } else {
+                    for (int j = 0; j < 8 && c + j < A.cols; ++j) q |= (uint32_t)(p[j / 2] >> (4 * (j & 1)) & 15) << (4 * j);
+                }
+            }
+            out[s] = pair_up(q);
         }
-        A.w[i] = out;
+        ((uint4 *)A.w)[i] = make_uint4(out[0], out[1], out[2], out[3]);
     }
     for (int64_t i = i0; i < A.entries; i += step) {
         const int64_t r = i % TR, gi = i / TR % A.groups, row = i / TR / A.groups * TR + r;
@@ -253,8 +300,15 @@ int launch(const void *kernel, const char *where, dim3 grid, int threads, void *
     return e == hipSuccess ? SPMM_HIP_OK : fail(SPMM_HIP_ERR_HIP, "%s launch: %s", where, hipGetErrorString(e));
 }
 
-template <typename T> const void *matvec_of(bool zeros) {
-    return zeros ? (const void *)matvec_kernel<T, true> : (const void *)matvec_kernel<T, false>;
+template <typename T, bool ZEROS, int RT> const void *matvec_sg(int group) {
+    return group >= 128 ? (const void *)matvec_kernel<T, ZEROS, RT, 1>
+           : group == 64 ? (const void *)matvec_kernel<T, ZEROS, RT, 2> : (const void *)matvec_kernel<T, ZEROS, RT, 4>;
+}
+template <typename T, bool ZEROS> const void *matvec_rt(int rt, int group) {
+    return rt == 4 ? matvec_sg<T, ZEROS, 4>(group) : rt == 2 ? matvec_sg<T, ZEROS, 2>(group) : matvec_sg<T, ZEROS, 1>(group);
+}
+template <typename T> const void *matvec_of(bool zeros, int rt, int group) {
+    return zeros ? matvec_rt<T, true>(rt, group) : matvec_rt<T, false>(rt, group);
 }
 
 }  // namespace
@@ -303,7 +357,8 @@ int spmm_q4_layout(const spmm_q4_desc_t *w, const void *packed, int64_t packed_s
     A.entries = s.row_tiles * s.groups * TR;
     A.tiles = (int)s.tiles;
     A.groups = (int)s.groups;
-    const int64_t blocks = (A.words + 255) / 256;
+    A.words_aligned = (uintptr_t)packed % 4 == 0 && packed_stride % 4 == 0;
+    const int64_t blocks = (A.words / 4 + 255) / 256;
     void *args[] = {&A};
     return launch(s.es == 4 ? (const void *)layout_kernel<float> : (const void *)layout_kernel<uint16_t>, W,
                   dim3((unsigned)(blocks < 8192 ? blocks : 8192)), 256, args, stream);
@@ -340,14 +395,18 @@ int spmm_q4_matvec(const spmm_q4_desc_t *w, const void *layout, const void *x, i
     A.row_tiles = (int)s.row_tiles;
     A.group = w->group;
     A.wide = (uintptr_t)x % 16 == 0 && (tokens == 1 || x_stride % (16 / s.es) == 0);
-    // waves share a row tile's columns: about 16 waves a compute unit in all, one column tile each at least
+    // Row tiles that share a block's x: as many as leave a block for every compute unit.  Waves that share the columns: 16 a
+    // compute unit in all, one column tile each at least.
+    const int rt = s.row_tiles >= 8 * 256 ? 4 : s.row_tiles >= 4 * 256 ? 2 : 1;
+    const int64_t blocks = (s.row_tiles + rt - 1) / rt;
     int waves = 1;
-    while (waves < WMAX && waves < A.tiles && s.row_tiles * waves < 4096) waves *= 2;
+    while (waves < WMAX && waves < A.tiles && blocks * waves < 4096) waves *= 2;
     const int per = w->dtype == SPMM_Q4_F32 ? 5 : 16;
     void *args[] = {&A};
-    const void *kern = w->dtype == SPMM_Q4_F32 ? matvec_of<float>(w->zeros)
-                       : w->dtype == SPMM_Q4_F16 ? matvec_of<_Float16>(w->zeros) : matvec_of<__bf16>(w->zeros);
-    return launch(kern, W, dim3((unsigned)s.row_tiles, (unsigned)((tokens + per - 1) / per)), waves * 64, args, stream);
+    const void *kern = w->dtype == SPMM_Q4_F32 ? matvec_of<float>(w->zeros, rt, w->group)
+                       : w->dtype == SPMM_Q4_F16 ? matvec_of<_Float16>(w->zeros, rt, w->group)
+                                                 : matvec_of<__bf16>(w->zeros, rt, w->group);
+    return launch(kern, W, dim3((unsigned)blocks, (unsigned)((tokens + per - 1) / per)), waves * 64, args, stream);
 }
 
 }  // extern "C"
