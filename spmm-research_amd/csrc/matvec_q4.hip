@@ -126,14 +126,21 @@ template <typename T, bool ZEROS, int RT, int SG> __global__ __launch_bounds__(W
     f32x4 y[RT];
 #pragma unroll
     for (int i = 0; i < RT; ++i) y[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    // past the last row tile the last one again
+    auto weights = [&](int t, uint4 (&w)[RT]) {
+#pragma unroll
+        for (int i = 0; i < RT; ++i) w[i] = A.w[((int64_t)min(rt0 + i, A.row_tiles - 1) * A.tiles + t) * 64 + lane];
+    };
+    uint4 ahead[RT];
+    if (wave < A.tiles) weights(wave, ahead);
     for (int t = wave; t < A.tiles; t += waves) {
-        // everything of the tile is asked for before anything is used; past the last row tile the last one again
+        // everything of the tile, and the next one's weights, is asked for before anything is used
         uint4 w[RT];
         t4 sc[RT][SG];
         uint32_t z[RT][SG];
         frag<T> xr[4];
 #pragma unroll
-        for (int i = 0; i < RT; ++i) w[i] = A.w[((int64_t)min(rt0 + i, A.row_tiles - 1) * A.tiles + t) * 64 + lane];
+        for (int i = 0; i < RT; ++i) w[i] = ahead[i];
 #pragma unroll
         for (int s = 0; s < 4; ++s) xr[s] = fetch_x<T>(A, tok, (int64_t)t * TC + s * 32 + g4 * 8, mine);
 #pragma unroll
@@ -145,6 +152,7 @@ template <typename T, bool ZEROS, int RT, int SG> __global__ __launch_bounds__(W
                 sc[i][g] = *(const t4 *)((const T *)A.scales + at);
                 z[i][g] = ZEROS ? A.zeros[at / 4] : 0x08080808u;
             }
+        if (t + waves < A.tiles) weights(t + waves, ahead);
         f32x4 c[RT], sx = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int i = 0; i < RT; ++i) c[i] = f32x4{0.f, 0.f, 0.f, 0.f};
