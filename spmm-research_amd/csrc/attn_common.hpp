@@ -222,6 +222,13 @@ template <typename T> __device__ __forceinline__ frag<T> load_frag(const T *src,
     return f;
 }
 
+// The fragments are in their registers from here on.  Without it the compiler puts the wait for these loads where they are
+// first used, in the loop, and there it waits on every turn for the tiles under way as well.
+template <typename T, int N> __device__ __forceinline__ void settled(frag<T> (&f)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) asm volatile("" : "+v"(f[i]));
+}
+
 // 4 consecutive results of a row
 template <typename T> __device__ __forceinline__ void store4(T *dst, int el, int dim, bool wide, f32x4 x) {
     typedef T t4 __attribute__((ext_vector_type(4)));

@@ -60,6 +60,7 @@ __global__ __launch_bounds__(256, 2) void window_kernel(WindowArgs A) {
             if (A.scale2 < 0.f) qf[st] = -qf[st];
             if (A.scale2 == 0.f) qf[st] = frag<T>{};
         }
+        settled<T>(qf);
     }
     const float scale2 = A.scale2 == 0.f ? 1.f : fabsf(A.scale2);
 

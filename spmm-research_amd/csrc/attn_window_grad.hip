@@ -77,11 +77,14 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void grad_q_kernel(Win
             qf[st] = load_frag<T>(qr, st * 16 + h * 8, A.dim, A.q.wide);
             df[st] = load_frag<T>(dr, st * 16 + h * 8, A.dim, A.dout.wide);
         }
+        settled<T>(qf);
+        settled<T>(df);
         if (mine) {
             const int64_t x = (packed ? s.q0 + i : s.b * A.q_len + i) * A.heads + head;
             lse2 = A.stats[2 * x];
             delta = A.stats[2 * x + 1];
         }
+        asm volatile("" : "+v"(lse2), "+v"(delta));
     }
     using Move = Mover<T, DP, GN, 256>;
     Move mk, mv;
@@ -248,6 +251,8 @@ __device__ __forceinline__ bool grad_kv_block(const WindowArgs &A, KvShared<T, D
             kf[st] = load_frag<T>(kr, st * 16 + h * 8, A.dim, A.k.wide);
             vf[st] = load_frag<T>(vr, st * 16 + h * 8, A.dim, A.v.wide);
         }
+        settled<T>(kf);
+        settled<T>(vf);
     }
     using Move = Mover<T, DP, GN, 256>;
     constexpr int LOADS = 2 * Move::N + 1;                           // of a tile, a wave
