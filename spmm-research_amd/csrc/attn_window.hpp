@@ -16,6 +16,7 @@ struct WindowArgs {
     int tiles, zero_rest;
     float *part;             // gradients: parts of the first keys' gradients
     int chunk;               // queries of a part, 0: not split
+    int block_keys;          // keys of a block of the kernel that owns keys
 };
 
 // Key head, query head inside its group, and tile of a block.  Consecutive blocks go round the eight dies, so

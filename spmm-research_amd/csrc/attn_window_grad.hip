@@ -192,141 +192,161 @@ __device__ __forceinline__ int window_end(const WindowArgs &A, const Seq &s, int
     return min(s.nq - 1, n1 + A.mask.window - 1 - (s.nk - s.nq));
 }
 
-constexpr int STAGES = 4;                    // tiles of queries on their way or in use
-
-template <typename T, int DP> struct KvShared {
-    __align__(16) T q[STAGES][GN * Tile<T, DP>::PITCH], d[STAGES][GN * Tile<T, DP>::PITCH];
-    __align__(16) float s[STAGES][2 * GN];                           // lse and D of the tile's rows
+// How a block of the kernel below is made up: KG groups of 32 keys, whose keys and values stay in LDS, times PG waves that
+// share a group's queries, 32 of every tile each, and add up in order at the end; STAGES tiles of 32 PG queries on
+// their way or in use.
+template <typename T, int DP, int KG, int PG> struct KvShape {
+    static constexpr int KEYS = 32 * KG, QN = 32 * PG, THREADS = 64 * KG * PG;
+    static constexpr int TILE = 2 * QN * Tile<T, DP>::PITCH * (int)sizeof(T) + 8 * QN;
+    static constexpr int KV = 2 * KEYS * Tile<T, DP>::PITCH * (int)sizeof(T);
+    static constexpr int STAGES = (160 * 1024 - 64 - KV) / TILE < 4 ? (160 * 1024 - 64 - KV) / TILE : 4;
+    static_assert(STAGES >= 1, "one tile has to fit");
+};
+template <typename T, int DP, int KG, int PG> struct KvShared {
+    using S = KvShape<T, DP, KG, PG>;
+    static constexpr int P = Tile<T, DP>::PITCH;
+    __align__(16) T k[S::KEYS * P], v[S::KEYS * P];                  // at the end: a wave's sums for another
+    __align__(16) T q[S::STAGES][S::QN * P], d[S::STAGES][S::QN * P];
+    __align__(16) float s[S::STAGES][2 * S::QN];                     // lse and D of the tile's rows
     int odd;
 };
 
 // False, with nothing written, if a value in a partly seen tile is not finite and CAREFUL does not allow for that.
-template <typename T, int DP, bool DIRECT, bool CAREFUL>
-__device__ __forceinline__ bool grad_kv_block(const WindowArgs &A, KvShared<T, DP> &sh) {
+template <typename T, int DP, int KG, int PG, bool DIRECT, bool CAREFUL>
+__device__ __forceinline__ bool grad_kv_block(const WindowArgs &A, KvShared<T, DP, KG, PG> &sh) {
     using L = Tile<T, DP>;
-    constexpr int ND = DP / 32, NS = DP / 16;
-    auto &sq = sh.q;
-    auto &sd = sh.d;
-    auto &ss = sh.s;
-    int &odd = sh.odd;
+    using S = KvShape<T, DP, KG, PG>;
+    constexpr int ND = DP / 32, NS = DP / 16, QN = S::QN, KEYS = S::KEYS, STAGES = S::STAGES, THREADS = S::THREADS;
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), h = lane >> 5;
-    int kv, g, t;
-    place(A, 1, &kv, &g, &t);
-    const bool packed = A.cu_q != nullptr;
-    const bool extra = t >= A.tiles;                                 // a chunk of queries for the first keys
-    const Seq s = extra ? find_tile(t - A.tiles, A.chunk, false, A.cu_q, A.cu_k, A.batch, A.q_len, A.k_len)
-                        : find_tile(t, GM, true, A.cu_q, A.cu_k, A.batch, A.q_len, A.k_len);
+    const int kg = wave % KG, part = wave / KG;                       // the wave's keys, and which queries of a tile
+    // the blocks that own keys, then those that take a chunk of queries for a block of the first keys each
+    const int ke = (A.mask.sinks + KEYS - 1) / KEYS;
+    int t = (int)blockIdx.x, e0 = 0;
+    const bool packed = A.cu_q != nullptr, extra = t >= A.tiles * A.kv_heads;
+    if (extra) t -= A.tiles * A.kv_heads;
+    const int kv = t % A.kv_heads;
+    t /= A.kv_heads;
+    if (extra) {
+        e0 = t % ke;
+        t /= ke;
+    }
+    const Seq s = extra ? find_tile(t, A.chunk, false, A.cu_q, A.cu_k, A.batch, A.q_len, A.k_len)
+                        : find_tile(t, KEYS, true, A.cu_q, A.cu_k, A.batch, A.q_len, A.k_len);
     if (s.tile < 0) {
         if (A.zero_rest && packed && !extra) {
-            const int64_t from = s.rest + (int64_t)(t - s.nq) * GM, step = (int64_t)(A.tiles - s.nq) * GM;
-            zero_rows<T>(A.dk, from, step, GM, A.k_len, kv, A.dim);
-            zero_rows<T>(A.dv, from, step, GM, A.k_len, kv, A.dim);
+            const int64_t from = s.rest + (int64_t)(t - s.nq) * KEYS, step = (int64_t)(A.tiles - s.nq) * KEYS;
+            zero_rows<T>(A.dk, from, step, KEYS, A.k_len, kv, A.dim);
+            zero_rows<T>(A.dv, from, step, KEYS, A.k_len, kv, A.dim);
         }
         return true;
     }
-    if (tid == 0) odd = 0;
+    if (tid == 0) sh.odd = 0;
     const int group = A.heads / A.kv_heads;
-    const int shift = s.nk - s.nq, n0 = extra ? 0 : s.tile * GM;
-    const int n1 = min(n0 + GM, extra ? min(A.mask.sinks, s.nk) : s.nk) - 1;
+    const int shift = s.nk - s.nq, n0 = (extra ? e0 : s.tile) * KEYS;
+    const int n1 = min(n0 + KEYS, extra ? min(A.mask.sinks, s.nk) : s.nk) - 1;
     const bool first = A.chunk > 0 && n0 < A.mask.sinks;            // the first keys' results go to `part`
     // queries that see some key of the block
     int i0 = max(0, n0 - shift);
     int i1 = A.mask.window == 0 || (n0 < A.mask.sinks && !first) ? s.nq - 1 : window_end(A, s, n1);
     if (extra) {
-        i0 = max(s.tile * A.chunk, window_end(A, s, min(GM, s.nk) - 1) + 1);
+        i0 = max(s.tile * A.chunk, window_end(A, s, min(n0 + KEYS, s.nk) - 1) + 1);
         i1 = min((s.tile + 1) * A.chunk, s.nq) - 1;
-        if (i1 < i0 || n1 < 0) return true;
+        if (i1 < i0 || n1 < n0) return true;
     }
-    const int q0t = i0 / GN, nqt = i1 >= i0 ? i1 / GN - q0t + 1 : 0, tiles = nqt * group;
+    const int first_j = i0 / QN * QN, per_head = i1 >= i0 ? (i1 - first_j) / QN + 1 : 0, tiles = per_head * group;
 
-    const int key = n0 + wave * 32 + (lane & 31);
+    const int key = n0 + kg * 32 + (lane & 31);
     const bool mine = key <= n1;
-    const int c0 = n0 + wave * 32, c1 = min(c0 + 31, n1);          // the wave's keys
-    frag<T> kf[NS], vf[NS];
-    {
-        const T *kr = mine ? seq_base<T>(A.k, s, s.k0, packed, kv) + key * A.k.row : nullptr;
-        const T *vr = mine ? seq_base<T>(A.v, s, s.k0, packed, kv) + key * A.v.row : nullptr;
-#pragma unroll
-        for (int st = 0; st < NS; ++st) {
-            kf[st] = load_frag<T>(kr, st * 16 + h * 8, A.dim, A.k.wide);
-            vf[st] = load_frag<T>(vr, st * 16 + h * 8, A.dim, A.v.wide);
-        }
-        settled<T>(kf);
-        settled<T>(vf);
-    }
-    using Move = Mover<T, DP, GN, 256>;
+    const T *kb = seq_base<T>(A.k, s, s.k0, packed, kv) + n0 * A.k.row, *vb = seq_base<T>(A.v, s, s.k0, packed, kv) + n0 * A.v.row;
+    using MoveK = Mover<T, DP, KEYS, THREADS>;
+    using Move = Mover<T, DP, QN, THREADS>;
     constexpr int LOADS = 2 * Move::N + 1;                           // of a tile, a wave
     Move mq, md;
     if (DIRECT) {
+        MoveK mk;
+        mk.start(tid, A.dim, A.k.row);
+        mk.send(wave, sh.k, kb, A.k.row, n1 + 1 - n0, A.dim);
+        mk.start(tid, A.dim, A.v.row);
+        mk.send(wave, sh.v, vb, A.v.row, n1 + 1 - n0, A.dim);
         mq.start(tid, A.dim, A.q.row);
         md.start(tid, A.dim, A.dout.row);
+    } else {
+        MoveK::copy(tid, A.dim, sh.k, [&](int r) { return n0 + r <= n1 ? kb + r * A.k.row : nullptr; });
+        MoveK::copy(tid, A.dim, sh.v, [&](int r) { return n0 + r <= n1 ? vb + r * A.v.row : nullptr; });
     }
-    const float *stats = A.stats + (packed ? s.q0 : s.b * A.q_len) * A.heads * 2;
-    // tile `it`: query tile q0t + it % nqt of the group's head it / nqt; beyond the last there are no rows
-    auto send = [&](int it, int buf) {
-        const int head = kv * group + min(it / max(nqt, 1), group - 1), j0 = (q0t + it % max(nqt, 1)) * GN;
-        const int rows = it < tiles ? s.nq - j0 : 0;
-        mq.send(wave, sq[buf], seq_base<T>(A.q, s, s.q0, packed, head) + (int64_t)j0 * A.q.row, A.q.row, rows, A.dim);
-        md.send(wave, sd[buf], seq_base<T>(A.dout, s, s.q0, packed, head) + (int64_t)j0 * A.dout.row, A.dout.row, rows, A.dim);
-        const int n = min(rows, GN);
-        const Buffer b(stats + ((int64_t)j0 * A.heads + head) * 2, n > 0 ? ((n - 1) * A.heads + 1) * 8 : 0);
-        b.to_lds4(ss[buf], (lane >> 1) * A.heads * 8 + (lane & 1) * 4);     // every wave alike: equal counts of loads
+    // The tile that is fetched next: the group's heads one after the other, the queries of each from first_j on.  Past the
+    // last there are no rows.
+    int next_left = tiles, next_j = first_j, next_g = 0;
+    const T *next_q = nullptr, *next_d = nullptr;
+    const float *next_s = nullptr;
+    auto rewind = [&] {
+        const int head = kv * group + next_g;
+        next_j = first_j;
+        next_q = seq_base<T>(A.q, s, s.q0, packed, head) + (int64_t)first_j * A.q.row;
+        next_d = seq_base<T>(A.dout, s, s.q0, packed, head) + (int64_t)first_j * A.dout.row;
+        next_s = A.stats + (((packed ? s.q0 : s.b * A.q_len) + first_j) * A.heads + head) * 2;
     };
-    auto copy = [&](int it, int buf) {
-        const int head = kv * group + it / nqt, j0 = (q0t + it % nqt) * GN;
-        const T *qb = seq_base<T>(A.q, s, s.q0, packed, head), *db = seq_base<T>(A.dout, s, s.q0, packed, head);
-        Move::copy(tid, A.dim, sq[buf], [&](int r) { return j0 + r < s.nq ? qb + (int64_t)(j0 + r) * A.q.row : nullptr; });
-        Move::copy(tid, A.dim, sd[buf], [&](int r) { return j0 + r < s.nq ? db + (int64_t)(j0 + r) * A.dout.row : nullptr; });
-        if (tid < 2 * GN) ss[buf][tid] = j0 + tid / 2 < s.nq ? stats[((int64_t)(j0 + tid / 2) * A.heads + head) * 2 + tid % 2] : 0.f;
+    if (tiles) rewind();
+    auto advance = [&]() __attribute__((always_inline)) {
+        next_q += QN * A.q.row;
+        next_d += QN * A.dout.row;
+        next_s += (int64_t)QN * A.heads * 2;
+        next_j += QN;
+        --next_left;
+        if (next_j > i1 && next_left > 0) {
+            ++next_g;
+            rewind();
+        }
+    };
+    auto fetch = [&](int buf) __attribute__((always_inline)) {
+        const int rows = next_left > 0 ? s.nq - next_j : 0;
+        if constexpr (DIRECT) {
+            mq.send(wave, sh.q[buf], next_q, A.q.row, rows, A.dim);
+            md.send(wave, sh.d[buf], next_d, A.dout.row, rows, A.dim);
+            // the rows of this wave's queries: every wave the same number of loads
+            const int n = max(0, min(rows - 32 * part, 32));
+            const Buffer b(next_s + (int64_t)32 * part * A.heads * 2, n > 0 ? ((n - 1) * A.heads + 1) * 8 : 0);
+            b.to_lds4(sh.s[buf] + 64 * part, (lane >> 1) * A.heads * 8 + (lane & 1) * 4);
+        } else {
+            Move::copy(tid, A.dim, sh.q[buf], [&](int r) { return r < rows ? next_q + r * A.q.row : nullptr; });
+            Move::copy(tid, A.dim, sh.d[buf], [&](int r) { return r < rows ? next_d + r * A.dout.row : nullptr; });
+            for (int e = tid; e < 2 * QN; e += THREADS) sh.s[buf][e] = e / 2 < rows ? next_s[(int64_t)(e / 2) * A.heads * 2 + e % 2] : 0.f;
+        }
+        advance();
     };
     f32x16 dk[ND], dv[ND];
     // the positions plo .. plo + seen - 1 are those of the block's queries that see this lane's key
     const int plo = max(key, i0 + shift);
     const int phi = min(i1 + shift, A.mask.window == 0 || key < A.mask.sinks ? INT32_MAX : key + A.mask.window - 1);
     const unsigned seen = (unsigned)max(0, phi - plo + 1);
+    // tiles that start in [all_a, all_b] are seen by every key of the block, the wave's 32 queries that start in [own_a, own_b]
+    // by every key of the wave
+    const int c0 = n0 + kg * 32, c1 = min(c0 + 31, n1);
+    auto last_for = [&](int a, int b) { return A.mask.window == 0 || b < A.mask.sinks ? i1 : min(i1, a + A.mask.window - 1 - shift); };
+    const int all_a = max(n1 - shift, i0), all_b = last_for(n0, n1) - QN + 1;
+    const int own_a = max(c1 - shift, i0), own_b = last_for(c0, c1) - 31;
     // rows behind the last query are zeros, lse and D too: P = 1 then, and adds 1 * 0
-    auto step = [&](int j0, const T *tq, const T *td, const float *ts) {
-        const int p0 = j0 + shift;
-        const bool full = A.mask.all(p0, p0 + GN - 1, c0, c1) && j0 >= i0 && j0 + GN - 1 <= i1;
-        // Every read from LDS is issued well before its product: the only wave of a SIMD has none to hide behind.
-        frag<T> ra[NS], rb[NS];
-#pragma unroll
-        for (int st = 0; st < NS; ++st) {
-            ra[st] = L::row_frag(tq, lane & 31, st * 16 + h * 8);
-            rb[st] = L::row_frag(td, lane & 31, st * 16 + h * 8);
-        }
-        f32x4 stat[8];
-#pragma unroll
-        for (int r = 0; r < 8; ++r) stat[r] = *reinterpret_cast<const f32x4 *>(ts + 2 * (row_of(2 * r) + 4 * h));
-        __builtin_amdgcn_sched_barrier(0);
+    auto step = [&](int j0, const T *tq, const T *td, const float *ts) __attribute__((always_inline)) {
         f32x16 sc = zero16(), dp = zero16();
 #pragma unroll
         for (int st = 0; st < NS; ++st) {
-            sc = mma32(ra[st], kf[st], sc);
-            dp = mma32(rb[st], vf[st], dp);
+            sc = mma32(L::row_frag(tq, lane & 31, st * 16 + h * 8), L::row_frag(sh.k, kg * 32 + (lane & 31), st * 16 + h * 8), sc);
+            dp = mma32(L::row_frag(td, lane & 31, st * 16 + h * 8), L::row_frag(sh.v, kg * 32 + (lane & 31), st * 16 + h * 8), dp);
         }
-        __builtin_amdgcn_sched_barrier(0);
-        frag<T> co[2][ND], cq[2][ND];
-        if constexpr (!CAREFUL) {
 #pragma unroll
-            for (int k2 = 0; k2 < 2; ++k2)
+        for (int r2 = 0; r2 < 16; r2 += 2) {
+            const f32x4 st = *reinterpret_cast<const f32x4 *>(ts + 2 * (row_of(r2) + 4 * h));
 #pragma unroll
-                for (int d = 0; d < ND; ++d) {
-                    co[k2][d] = L::col_frag(td, k2 * 16, d * 32, lane);
-                    cq[k2][d] = L::col_frag(tq, k2 * 16, d * 32, lane);
-                }
+            for (int r = r2; r < r2 + 2; ++r) {
+                sc[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[r], A.scale2, -st[2 * (r - r2)]));
+                dp[r] = sc[r] * (dp[r] - st[2 * (r - r2) + 1]);
+            }
         }
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            sc[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[r], A.scale2, -stat[r / 2][2 * (r % 2)]));
-            dp[r] = sc[r] * (dp[r] - stat[r / 2][2 * (r % 2) + 1]);
-        }
-        if (!full) {
-            asm volatile("");
+        if (j0 < own_a || j0 > own_b) {
+            asm volatile("");                        // a branch, not 16 selects in every tile
 #pragma unroll
             for (int r = 0; r < 16; ++r)
-                if ((unsigned)(p0 + row_of(r) + 4 * h - plo) >= seen) sc[r] = dp[r] = 0.f;
+                if ((unsigned)(j0 + shift + row_of(r) + 4 * h - plo) >= seen) sc[r] = dp[r] = 0.f;
         }
         if constexpr (!CAREFUL) {
 #pragma unroll
@@ -334,49 +354,83 @@ __device__ __forceinline__ bool grad_kv_block(const WindowArgs &A, KvShared<T, D
                 const frag<T> pf = next_operand<T>(sc, k2), dsf = next_operand<T>(dp, k2);
 #pragma unroll
                 for (int d = 0; d < ND; ++d) {
-                    dv[d] = mma32(co[k2][d], pf, dv[d]);
-                    dk[d] = mma32(cq[k2][d], dsf, dk[d]);
+                    dv[d] = mma32(L::col_frag(td, k2 * 16, d * 32, lane), pf, dv[d]);
+                    dk[d] = mma32(L::col_frag(tq, k2 * 16, d * 32, lane), dsf, dk[d]);
                 }
             }
         } else {
             // a query that is not finite has an lse that is not, so its weights are NaN: it need not be put back
-            Careful<T, DP, GN> c;
+            Careful<T, DP, 32> c;
             for (int d = 0; d < ND; ++d) c.acc[d] = dv[d];
             c.w[0] = sc;
-            careful_product<T, DP, GN>(&c, td, lane, A.mask, key, p0, false, i1 + shift);
+            careful_product<T, DP, 32>(&c, td, lane, A.mask, key, j0 + shift, false, i1 + shift);
             for (int d = 0; d < ND; ++d) dv[d] = c.acc[d];
             for (int d = 0; d < ND; ++d) c.acc[d] = dk[d];
             c.w[0] = dp;
-            careful_product<T, DP, GN>(&c, tq, lane, A.mask, key, p0, false, INT32_MIN);
+            careful_product<T, DP, 32>(&c, tq, lane, A.mask, key, j0 + shift, false, INT32_MIN);
             for (int d = 0; d < ND; ++d) dk[d] = c.acc[d];
         }
     };
 #pragma unroll
     for (int d = 0; d < ND; ++d) dk[d] = dv[d] = zero16();
-    __syncthreads();
+    constexpr bool AHEAD = DIRECT && STAGES > 1;
     if (DIRECT) {
+        arrived();                                   // keys and values
+        if (AHEAD) {
 #pragma unroll
-        for (int it = 0; it < STAGES - 1; ++it) send(it, it);
+            for (int it = 0; it < STAGES - 1; ++it) fetch(it);
+        }
     }
+    __syncthreads();
     bool fine = true;
-    for (int it = 0; it < tiles; ++it) {
-        const int buf = it % STAGES, j0 = (q0t + it % nqt) * GN, p0 = j0 + shift;
-        if (DIRECT) arrived<(STAGES - 2) * LOADS>();
-        else copy(it, buf);
-        const bool whole = A.mask.all(p0, p0 + GN - 1, n0, n1) && j0 >= i0 && j0 + GN - 1 <= i1;
-        if (!whole && (Move::any_not_finite(tid, sq[buf]) || Move::any_not_finite(tid, sd[buf]))) odd = 1;
+    for (int it = 0, j0 = first_j, buf = 0; it < tiles; ++it) {
+        if (AHEAD) {
+            arrived<(STAGES - 2) * LOADS>();
+        } else {
+            fetch(buf);
+            if (DIRECT) arrived();
+        }
+        const bool whole = j0 >= all_a && j0 <= all_b;
+        if (!whole && (Move::any_not_finite(tid, sh.q[buf]) || Move::any_not_finite(tid, sh.d[buf]))) sh.odd = 1;
         __syncthreads();                             // tile `it` is there for all, and tile `it` - 1 is read
-        if (!CAREFUL && !whole && uniform(odd)) {    // the whole block leaves at the same tile
+        if (!CAREFUL && !whole && uniform(sh.odd)) {  // the whole block leaves at the same tile
             fine = false;
             break;
         }
-        if (DIRECT) send(it + STAGES - 1, (it + STAGES - 1) % STAGES);
-        step(j0, sq[buf], sd[buf], ss[buf]);
-        if (!DIRECT) __syncthreads();
+        if (AHEAD) fetch(buf == 0 ? STAGES - 1 : buf - 1);
+        step(j0 + 32 * part, sh.q[buf] + 32 * part * L::PITCH, sh.d[buf] + 32 * part * L::PITCH, sh.s[buf] + 64 * part);
+        if (!AHEAD) __syncthreads();
+        if (AHEAD) buf = buf == STAGES - 1 ? 0 : buf + 1;
+        j0 += QN;
+        if (j0 > i1) j0 = first_j;
     }
     if (DIRECT) arrived();
     if (!fine) return false;
-    if (!mine) return true;
+    if constexpr (PG > 1) {                          // the parts' sums, in order, through the keys' place in LDS
+        float *mail = reinterpret_cast<float *>(sh.k) + kg * ND * 16 * 64 + lane;
+        auto pass = [&](f32x16 (&x)[ND]) {
+#pragma unroll 1
+            for (int from = 1; from < PG; ++from) {
+                __syncthreads();
+                if (part == from) {
+#pragma unroll
+                    for (int d = 0; d < ND; ++d)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) mail[(d * 16 + r) * 64] = x[d][r];
+                }
+                __syncthreads();
+                if (part == 0) {
+#pragma unroll
+                    for (int d = 0; d < ND; ++d)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) x[d][r] += mail[(d * 16 + r) * 64];
+                }
+            }
+        };
+        pass(dk);
+        pass(dv);
+    }
+    if (!mine || part != 0) return true;
     if (first && key < A.mask.sinks) {
         float *pk = part_of(A, extra ? chunk_slot(A, s, packed, s.tile) : s.b, kv) + key * A.dim, *pv = pk + A.mask.sinks * A.dim;
 #pragma unroll
@@ -404,16 +458,17 @@ __device__ __forceinline__ bool grad_kv_block(const WindowArgs &A, KvShared<T, D
     return true;
 }
 // The rare case in a function of its own, which takes no registers from the loop above.
-template <typename T, int DP>
-__device__ __attribute__((noinline)) void grad_kv_again(const WindowArgs *A, KvShared<T, DP> *sh) {
-    grad_kv_block<T, DP, false, true>(*A, *sh);
+template <typename T, int DP, int KG, int PG>
+__device__ __attribute__((noinline)) void grad_kv_again(const WindowArgs *A, KvShared<T, DP, KG, PG> *sh) {
+    grad_kv_block<T, DP, KG, PG, false, true>(*A, *sh);
 }
-template <typename T, int DP, bool DIRECT> __global__ __launch_bounds__(256, 1) void grad_kv_kernel(WindowArgs A) {
-    __shared__ KvShared<T, DP> sh;
-    if (!grad_kv_block<T, DP, DIRECT, false>(A, sh)) {
+template <typename T, int DP, int KG, int PG, bool DIRECT>
+__global__ __launch_bounds__(64 * KG * PG, sizeof(T) == 2 ? 2 : 1) void grad_kv_kernel(WindowArgs A) {
+    __shared__ KvShared<T, DP, KG, PG> sh;
+    if (!grad_kv_block<T, DP, KG, PG, DIRECT, false>(A, sh)) {
         __syncthreads();
         const WindowArgs copy = A;
-        grad_kv_again<T, DP>(&copy, &sh);
+        grad_kv_again<T, DP, KG, PG>(&copy, &sh);
     }
 }
 
@@ -437,7 +492,7 @@ template <typename T> __global__ __launch_bounds__(64) void join_kernel(WindowAr
         s.nk = (int)A.k_len;
     }
     if (key >= s.nk) return;
-    const int end = window_end(A, s, min(GM, s.nk) - 1);
+    const int end = window_end(A, s, min((key / A.block_keys + 1) * A.block_keys, s.nk) - 1);      // of the key's block
     for (int e = threadIdx.x; e < 2 * A.dim; e += 64) {
         const int64_t x = (int64_t)(e / A.dim * A.mask.sinks + key) * A.dim + e % A.dim;       // keys' gradients, then values'
         float sum = part_of(A, b, kv)[x];
@@ -449,16 +504,33 @@ template <typename T> __global__ __launch_bounds__(64) void join_kernel(WindowAr
     }
 }
 
-struct GradKernels { const void *delta, *q, *kv, *join; };
-template <typename T, int DP> static GradKernels grads_for(bool direct_q, bool direct_kv) {
-    return {(const void *)delta_kernel<T>,
-            direct_q ? (const void *)grad_q_kernel<T, DP, true> : (const void *)grad_q_kernel<T, DP, false>,
-            direct_kv ? (const void *)grad_kv_kernel<T, DP, true> : (const void *)grad_kv_kernel<T, DP, false>,
-            (const void *)join_kernel<T>};
+struct GradKernels {
+    const void *delta, *q, *kv, *join;
+    int keys, threads;                       // of a block of kv
+};
+template <typename T, int DP, int KG, int PG> static void use_kv(GradKernels &g, bool direct) {
+    g.kv = direct ? (const void *)grad_kv_kernel<T, DP, KG, PG, true> : (const void *)grad_kv_kernel<T, DP, KG, PG, false>;
+    g.keys = KvShape<T, DP, KG, PG>::KEYS;
+    g.threads = KvShape<T, DP, KG, PG>::THREADS;
 }
-template <typename T> static GradKernels grads_of(int dim, bool direct_q, bool direct_kv) {
-    return dim <= 64 ? grads_for<T, 64>(direct_q, direct_kv) : dim <= 96 ? grads_for<T, 96>(direct_q, direct_kv)
-                                                                        : grads_for<T, 128>(direct_q, direct_kv);
+// few: there are not enough keys for a block of the large shape on every compute unit; blocks of 32 keys then, whose waves
+// share out the queries.
+template <typename T, int DP> static GradKernels grads_for(bool direct_q, bool direct_kv, bool few) {
+    GradKernels g = {(const void *)delta_kernel<T>,
+                     direct_q ? (const void *)grad_q_kernel<T, DP, true> : (const void *)grad_q_kernel<T, DP, false>, nullptr,
+                     (const void *)join_kernel<T>, 0, 0};
+    if constexpr (sizeof(T) == 2) {
+        if (few) use_kv<T, DP, 1, 4>(g, direct_kv);
+        else use_kv<T, DP, 4, 2>(g, direct_kv);
+    } else {
+        if (few) use_kv<T, DP, 1, DP == 64 ? 4 : 2>(g, direct_kv);
+        else use_kv<T, DP, 2, 2>(g, direct_kv);
+    }
+    return g;
+}
+template <typename T> static GradKernels grads_of(int dim, bool direct_q, bool direct_kv, bool few) {
+    return dim <= 64 ? grads_for<T, 64>(direct_q, direct_kv, few) : dim <= 96 ? grads_for<T, 96>(direct_q, direct_kv, few)
+                                                                             : grads_for<T, 128>(direct_q, direct_kv, few);
 }
 
 // Workspace: two floats a query row and head, then the first keys' parts where they are split.
@@ -528,19 +600,22 @@ extern "C" int spmm_attn_window_grad(const spmm_attn_desc_t *a, const spmm_attn_
     A.chunk = w.chunk;
     int qt = 0, kt = 0, ct = 0;
     if (a->q_len > 0 && (st = tile_count(a, W, packed, a->q_len, GM, &qt))) return st;
-    if (a->k_len > 0 && (st = tile_count(a, W, packed, a->k_len, GM, &kt))) return st;
+    const bool direct = A.k.direct && A.v.direct, direct_kv = direct && A.q.direct && A.dout.direct;
+    const bool few = (nb * a->k_len + 127) / 128 * a->kv_heads < 256;
+    const GradKernels G = a->dtype == SPMM_ATTN_F32 ? grads_of<float>(a->dim, direct, direct_kv, few)
+                          : a->dtype == SPMM_ATTN_F16 ? grads_of<_Float16>(a->dim, direct, direct_kv, few)
+                                                      : grads_of<__bf16>(a->dim, direct, direct_kv, few);
+    A.block_keys = G.keys;
+    if (a->k_len > 0 && (st = tile_count(a, W, packed, a->k_len, G.keys, &kt))) return st;
     if (w.chunk && (st = tile_count(a, W, packed, a->q_len, w.chunk, &ct))) return st;
     OnDevice on(a->device, W);
     if (on.status) return on.status;
-    const bool dq_direct = A.k.direct && A.v.direct, dkv_direct = A.q.direct && A.dout.direct;
-    const GradKernels G = a->dtype == SPMM_ATTN_F32 ? grads_of<float>(a->dim, dq_direct, dkv_direct)
-                          : a->dtype == SPMM_ATTN_F16 ? grads_of<_Float16>(a->dim, dq_direct, dkv_direct)
-                                                      : grads_of<__bf16>(a->dim, dq_direct, dkv_direct);
     void *args[] = {&A};
     const int64_t rows = nb * a->q_len * a->heads;
     if ((st = launch(G.delta, W, (rows + 15) / 16, 256, args, stream))) return st;
     A.tiles = kt;
-    if ((st = launch(G.kv, W, ((int64_t)kt + ct) * a->kv_heads, 256, args, stream))) return st;
+    const int64_t extra = w.chunk ? (int64_t)ct * ((A.mask.sinks + G.keys - 1) / G.keys) : 0;
+    if ((st = launch(G.kv, W, (kt + extra) * a->kv_heads, G.threads, args, stream))) return st;
     if (w.chunk && (st = launch(G.join, W, a->batch * a->kv_heads * A.mask.sinks, 64, args, stream))) return st;
     A.tiles = qt;
     return launch(G.q, W, (int64_t)qt * a->heads, 256, args, stream);
