@@ -9,18 +9,24 @@
 
 namespace attn {
 
-template <typename T> constexpr int BN_OF = sizeof(T) == 2 ? 64 : 32;      // keys of a tile
-constexpr int BM = 128;                                                      // queries of a workgroup
+// How a block is made up: MG groups of 32 queries times PG waves that share a group's keys, 32 SUB of every tile each, and
+// join at the end; two tiles of 32 PG SUB keys on their way or in use.
+template <typename T, int DP, int MG, int PG, int SUB> struct WindowShape {
+    static constexpr int ROWS = 32 * MG, BN = 32 * PG * SUB, THREADS = 64 * MG * PG;
+};
 constexpr float SLACK = 8.f;
 
-template <typename T, int DP, bool DIRECT>
-__global__ __launch_bounds__(256, 2) void window_kernel(WindowArgs A) {
+template <typename T, int DP, int MG, int PG, int SUB, bool DIRECT>
+__global__ __launch_bounds__(64 * MG * PG, sizeof(T) == 2 && PG == 1 ? 2 : 1) void window_kernel(WindowArgs A) {
     using L = Tile<T, DP>;
-    constexpr int BN = BN_OF<T>, ND = DP / 32, NS = DP / 16, NK = BN / 32;
+    using S = WindowShape<T, DP, MG, PG, SUB>;
+    constexpr int BM = S::ROWS, BN = S::BN, THREADS = S::THREADS, ND = DP / 32, NS = DP / 16, NK = SUB;
     __shared__ __align__(16) T sk[2][BN * L::PITCH], sv[2][BN * L::PITCH];
+    __shared__ float sm[PG > 1 ? PG * MG * 32 : 1];  // the parts' maxima
     __shared__ int odd;                              // some staged value of a partly visible tile was not finite
 
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
+    const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), h = lane >> 5;
+    const int mg = wave % MG, part = wave / MG;      // the wave's queries, and which keys of a tile
     int kv, g, t;
     place(A, A.heads / A.kv_heads, &kv, &g, &t);
     t = A.tiles - 1 - t;                             // late queries see more keys: they start first
@@ -47,9 +53,9 @@ __global__ __launch_bounds__(256, 2) void window_kernel(WindowArgs A) {
     auto tile_at = [&](int i) { return (i < ns ? i : lt + i - ns) * BN; };
 
     const T *kb = seq_base<T>(A.k, s, s.k0, packed, kv), *vb = seq_base<T>(A.v, s, s.k0, packed, kv);
-    const int i = m0 + wave * 32 + (lane & 31), p = i + shift;            // this lane's query
+    const int i = m0 + mg * 32 + (lane & 31), p = i + shift;              // this lane's query
     const bool mine = i < s.nq;
-    const int w0 = m0 + wave * 32 + shift, w1 = min(w0 + 31, pmax);       // the wave's positions
+    const int w0 = m0 + mg * 32 + shift, w1 = min(w0 + 31, pmax);         // the wave's positions
     frag<T> qf[NS];
     {
         const T *qr = mine ? seq_base<T>(A.q, s, s.q0, packed, head) + i * A.q.row : nullptr;
@@ -64,7 +70,7 @@ __global__ __launch_bounds__(256, 2) void window_kernel(WindowArgs A) {
     }
     const float scale2 = A.scale2 == 0.f ? 1.f : fabsf(A.scale2);
 
-    using Move = Mover<T, DP, BN, 256>;
+    using Move = Mover<T, DP, BN, THREADS>;
     Move mk, mv;
     if (DIRECT) {
         mk.start(tid, A.dim, A.k.row);
@@ -93,7 +99,7 @@ __global__ __launch_bounds__(256, 2) void window_kernel(WindowArgs A) {
     auto step = [&](auto careful, int j0, const T *tk, const T *tv) {
         // A wave whose queries see none of the block's tile goes through it all the same: a way round it would have the
         // accumulators copied at the end of every turn.
-        const bool full = A.mask.all(w0, w1, j0, j0 + BN - 1);
+        const bool full = A.mask.all(w0, w1, j0, j0 + 32 * SUB - 1);
         f32x16 sc[NK];
 #pragma unroll
         for (int n = 0; n < NK; ++n) {
@@ -147,10 +153,10 @@ __global__ __launch_bounds__(256, 2) void window_kernel(WindowArgs A) {
                         o[d] = mma32(L::col_frag(tv, n * 32 + k2 * 16, d * 32, lane), pf, o[d]);
                 }
         } else {
-            Careful<T, DP, BN> c;
+            Careful<T, DP, 32 * SUB> c;
             for (int d = 0; d < ND; ++d) c.acc[d] = o[d];
             for (int n = 0; n < NK; ++n) c.w[n] = sc[n];
-            careful_product<T, DP, BN>(&c, tv, lane, A.mask, p, j0, true, INT32_MAX);
+            careful_product<T, DP, 32 * SUB>(&c, tv, lane, A.mask, p, j0, true, INT32_MAX);
             for (int d = 0; d < ND; ++d) o[d] = c.acc[d];
         }
     };
@@ -171,7 +177,7 @@ __global__ __launch_bounds__(256, 2) void window_kernel(WindowArgs A) {
             if (!careful && !A.mask.all(pmin, pmax, j0, j0 + BN - 1) && uniform(odd)) return false;
             const bool more = it + 1 < tiles;
             if (DIRECT && more) send(tile_at(it + 1), sk[buf ^ 1], sv[buf ^ 1]);
-            step(careful, j0, sk[buf], sv[buf]);
+            step(careful, j0 + 32 * SUB * part, sk[buf] + 32 * SUB * part * L::PITCH, sv[buf] + 32 * SUB * part * L::PITCH);
             if (more) settle(tile_at(it + 1), sk[buf ^ 1], sv[buf ^ 1]);
             __syncthreads();
         }
@@ -183,7 +189,43 @@ __global__ __launch_bounds__(256, 2) void window_kernel(WindowArgs A) {
         run(std::true_type{});
     }
     sum += __shfl_xor(sum, 32);
-    if (!mine) return;
+    if constexpr (PG > 1) {                          // the parts, in order, through the tiles' place in LDS
+        float *mail = reinterpret_cast<float *>(sk) + mg * ND * 16 * 64 + lane;
+        sm[(part * MG + mg) * 32 + (lane & 31)] = m;
+        __syncthreads();
+        float top = m;
+#pragma unroll
+        for (int q = 0; q < PG; ++q) top = fmaxf(top, sm[(q * MG + mg) * 32 + (lane & 31)]);
+        const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
+        m = top;
+        sum *= f;
+#pragma unroll
+        for (int d = 0; d < ND; ++d) o[d] *= f;
+#pragma unroll 1
+        for (int from = 1; from < PG; ++from) {
+            if (from > 1) __syncthreads();
+            if (part == from) {
+#pragma unroll
+                for (int d = 0; d < ND; ++d)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) mail[(d * 16 + r) * 64] = o[d][r];
+            }
+            __syncthreads();
+            if (part == 0) {
+#pragma unroll
+                for (int d = 0; d < ND; ++d)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) o[d][r] += mail[(d * 16 + r) * 64];
+            }
+        }
+        __syncthreads();
+        sm[(part * MG + mg) * 32 + (lane & 31)] = sum;
+        __syncthreads();
+        sum = 0.f;
+#pragma unroll
+        for (int q = 0; q < PG; ++q) sum += sm[(q * MG + mg) * 32 + (lane & 31)];
+    }
+    if (!mine || part != 0) return;
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
     T *dst = seq_base<T>(A.out, s, s.q0, packed, head) + i * A.out.row;
 #pragma unroll
@@ -228,12 +270,20 @@ int tile_count(const spmm_attn_desc_t *a, const char *where, bool packed, int64_
     return SPMM_HIP_OK;
 }
 
-template <typename T, bool DIRECT> static const void *window_by(int dim) {
-    return dim <= 64 ? (const void *)window_kernel<T, 64, DIRECT> : dim <= 96 ? (const void *)window_kernel<T, 96, DIRECT>
-                                                                              : (const void *)window_kernel<T, 128, DIRECT>;
+struct WindowKernel { const void *kernel; int rows, threads; };
+template <typename T, int DP, int MG, int PG, int SUB> static WindowKernel window_with(bool direct) {
+    using S = WindowShape<T, DP, MG, PG, SUB>;
+    return {direct ? (const void *)window_kernel<T, DP, MG, PG, SUB, true> : (const void *)window_kernel<T, DP, MG, PG, SUB, false>,
+            S::ROWS, S::THREADS};
 }
-template <typename T> static const void *window_of(int dim, bool direct) {
-    return direct ? window_by<T, true>(dim) : window_by<T, false>(dim);
+template <typename T, int DP> static WindowKernel window_for(bool direct, bool few) {
+    if constexpr (sizeof(T) == 2) return few ? window_with<T, DP, 1, 4, 1>(direct) : window_with<T, DP, 4, 1, 2>(direct);
+    else return few ? window_with<T, DP, 1, DP == 64 ? 4 : 2, 1>(direct) : window_with<T, DP, 4, 1, 1>(direct);
+}
+// few: there are not enough queries for a block of the large shape on every compute unit; blocks of 32 queries then, whose
+// waves share out the keys.
+template <typename T> static WindowKernel window_of(int dim, bool direct, bool few) {
+    return dim <= 64 ? window_for<T, 64>(direct, few) : dim <= 96 ? window_for<T, 96>(direct, few) : window_for<T, 128>(direct, few);
 }
 
 }  // namespace attn
@@ -258,12 +308,12 @@ extern "C" int spmm_attn_window(const spmm_attn_desc_t *a, const spmm_attn_rows_
     if (nb == 0 || a->q_len == 0 || a->batch == 0) return SPMM_HIP_OK;
     if (!lse || (uintptr_t)lse % 4) return fail(SPMM_HIP_ERR_ARG, "%s: lse is NULL or not aligned", W);
     A.lse = lse;
-    if ((st = tile_count(a, W, packed, a->q_len, BM, &A.tiles))) return st;
+    const bool direct = A.k.direct && A.v.direct, few = (nb * a->q_len + 127) / 128 * a->heads < 256;
+    const WindowKernel K = a->dtype == SPMM_ATTN_F32 ? window_of<float>(a->dim, direct, few)
+                           : a->dtype == SPMM_ATTN_F16 ? window_of<_Float16>(a->dim, direct, few) : window_of<__bf16>(a->dim, direct, few);
+    if ((st = tile_count(a, W, packed, a->q_len, K.rows, &A.tiles))) return st;
     OnDevice on(a->device, W);
     if (on.status) return on.status;
-    const bool direct = A.k.direct && A.v.direct;
-    const void *kern = a->dtype == SPMM_ATTN_F32 ? window_of<float>(a->dim, direct)
-                       : a->dtype == SPMM_ATTN_F16 ? window_of<_Float16>(a->dim, direct) : window_of<__bf16>(a->dim, direct);
     void *args[] = {&A};
-    return launch(kern, W, (int64_t)A.tiles * a->heads, 256, args, stream);
+    return launch(K.kernel, W, (int64_t)A.tiles * a->heads, K.threads, args, stream);
 }

@@ -33,16 +33,21 @@ template <typename T> __global__ __launch_bounds__(256) void delta_kernel(Window
     }
 }
 
-constexpr int GM = 128;                      // rows a workgroup owns, 32 a wave
-constexpr int GN = 32;                       // rows of a staged tile
+// How a block is made up: as in the forward kernel, MG groups of 32 queries times PG waves that share a group's keys, 32 SUB
+// of every tile each.
+template <typename T, int DP, int MG, int PG, int SUB> struct QShape {
+    static constexpr int ROWS = 32 * MG, KN = 32 * PG * SUB, THREADS = 64 * MG * PG;
+};
 
-template <typename T, int DP, bool DIRECT>
-__global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void grad_q_kernel(WindowArgs A) {
+template <typename T, int DP, int MG, int PG, int SUB, bool DIRECT>
+__global__ __launch_bounds__(64 * MG * PG, sizeof(T) == 2 && PG == 1 ? 2 : 1) void grad_q_kernel(WindowArgs A) {
     using L = Tile<T, DP>;
-    constexpr int ND = DP / 32, NS = DP / 16;
+    using S = QShape<T, DP, MG, PG, SUB>;
+    constexpr int GM = S::ROWS, GN = S::KN, THREADS = S::THREADS, ND = DP / 32, NS = DP / 16;
     __shared__ __align__(16) T sk[2][GN * L::PITCH], sv[2][GN * L::PITCH];
     __shared__ int odd;
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), h = lane >> 5;
+    const int mg = wave % MG, part = wave / MG;      // the wave's queries, and which keys of a tile
     int kv, g, t;
     place(A, A.heads / A.kv_heads, &kv, &g, &t);
     t = A.tiles - 1 - t;
@@ -64,9 +69,9 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void grad_q_kernel(Win
     auto tile_at = [&](int i) { return (i < ns ? i : lt + i - ns) * GN; };
 
     const T *kb = seq_base<T>(A.k, s, s.k0, packed, kv), *vb = seq_base<T>(A.v, s, s.k0, packed, kv);
-    const int i = m0 + wave * 32 + (lane & 31), p = i + shift;
+    const int i = m0 + mg * 32 + (lane & 31), p = i + shift;
     const bool mine = i < s.nq;
-    const int w0 = m0 + wave * 32 + shift, w1 = min(w0 + 31, pmax);
+    const int w0 = m0 + mg * 32 + shift, w1 = min(w0 + 31, pmax);
     frag<T> qf[NS], df[NS];
     float lse2 = INFINITY, delta = 0.f;          // a row that is not there, or sees nothing: exp2(x - inf) = 0
     {
@@ -86,7 +91,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void grad_q_kernel(Win
         }
         asm volatile("" : "+v"(lse2), "+v"(delta));
     }
-    using Move = Mover<T, DP, GN, 256>;
+    using Move = Mover<T, DP, GN, THREADS>;
     Move mk, mv;
     if (DIRECT) {
         mk.start(tid, A.dim, A.k.row);
@@ -109,8 +114,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void grad_q_kernel(Win
         if (!A.mask.all(pmin, pmax, j0, j0 + GN - 1) && Move::any_not_finite(tid, tk)) odd = 1;
     };
     f32x16 dq[ND];
-    auto step = [&](auto careful, int j0, const T *tk, const T *tv) {
-        const bool full = A.mask.all(w0, w1, j0, j0 + GN - 1);
+    auto step = [&](auto careful, int j0, const T *tk, const T *tv) __attribute__((always_inline)) {
+        const bool full = A.mask.all(w0, w1, j0, j0 + 31);
         f32x16 sc = zero16(), dp = zero16();
 #pragma unroll
         for (int st = 0; st < NS; ++st) {
@@ -135,10 +140,10 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void grad_q_kernel(Win
                 for (int d = 0; d < ND; ++d) dq[d] = mma32(L::col_frag(tk, k2 * 16, d * 32, lane), dsf, dq[d]);
             }
         } else {
-            Careful<T, DP, GN> c;
+            Careful<T, DP, 32> c;
             for (int d = 0; d < ND; ++d) c.acc[d] = dq[d];
             c.w[0] = sc;
-            careful_product<T, DP, GN>(&c, tk, lane, A.mask, p, j0, true, -1);
+            careful_product<T, DP, 32>(&c, tk, lane, A.mask, p, j0, true, -1);
             for (int d = 0; d < ND; ++d) dq[d] = c.acc[d];
         }
     };
@@ -156,7 +161,11 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void grad_q_kernel(Win
             if (!careful && !A.mask.all(pmin, pmax, j0, j0 + GN - 1) && uniform(odd)) return false;
             const bool more = it + 1 < tiles;
             if (DIRECT && more) send(tile_at(it + 1), sk[buf ^ 1], sv[buf ^ 1]);
-            step(careful, j0, sk[buf], sv[buf]);
+#pragma unroll
+            for (int u = 0; u < SUB; ++u) {
+                const int r = 32 * (SUB * part + u);
+                step(careful, j0 + r, sk[buf] + r * L::PITCH, sv[buf] + r * L::PITCH);
+            }
             if (more) settle(tile_at(it + 1), sk[buf ^ 1], sv[buf ^ 1]);
             __syncthreads();
         }
@@ -167,7 +176,27 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void grad_q_kernel(Win
         __syncthreads();
         run(std::true_type{});
     }
-    if (!mine) return;
+    if constexpr (PG > 1) {                          // the parts' sums, in order, through the tiles' place in LDS
+        float *mail = reinterpret_cast<float *>(sk) + mg * ND * 16 * 64 + lane;
+#pragma unroll 1
+        for (int from = 1; from < PG; ++from) {
+            if (from > 1) __syncthreads();
+            if (part == from) {
+#pragma unroll
+                for (int d = 0; d < ND; ++d)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) mail[(d * 16 + r) * 64] = dq[d][r];
+            }
+            __syncthreads();
+            if (part == 0) {
+#pragma unroll
+                for (int d = 0; d < ND; ++d)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) dq[d][r] += mail[(d * 16 + r) * 64];
+            }
+        }
+    }
+    if (!mine || part != 0) return;
     T *dst = seq_base<T>(A.dq, s, s.q0, packed, head) + i * A.dq.row;
 #pragma unroll
     for (int d = 0; d < ND; ++d)
@@ -463,7 +492,7 @@ __device__ __attribute__((noinline)) void grad_kv_again(const WindowArgs *A, KvS
     grad_kv_block<T, DP, KG, PG, false, true>(*A, *sh);
 }
 template <typename T, int DP, int KG, int PG, bool DIRECT>
-__global__ __launch_bounds__(64 * KG * PG, sizeof(T) == 2 ? 2 : 1) void grad_kv_kernel(WindowArgs A) {
+__global__ __launch_bounds__(64 * KG * PG, KG * PG == 8 ? 2 : 1) void grad_kv_kernel(WindowArgs A) {
     __shared__ KvShared<T, DP, KG, PG> sh;
     if (!grad_kv_block<T, DP, KG, PG, DIRECT, false>(A, sh)) {
         __syncthreads();
@@ -506,31 +535,35 @@ template <typename T> __global__ __launch_bounds__(64) void join_kernel(WindowAr
 
 struct GradKernels {
     const void *delta, *q, *kv, *join;
-    int keys, threads;                       // of a block of kv
+    int keys, threads, q_rows, q_threads;    // of a block of kv and of q
 };
 template <typename T, int DP, int KG, int PG> static void use_kv(GradKernels &g, bool direct) {
     g.kv = direct ? (const void *)grad_kv_kernel<T, DP, KG, PG, true> : (const void *)grad_kv_kernel<T, DP, KG, PG, false>;
     g.keys = KvShape<T, DP, KG, PG>::KEYS;
     g.threads = KvShape<T, DP, KG, PG>::THREADS;
 }
+template <typename T, int DP, int MG, int PG, int SUB> static void use_q(GradKernels &g, bool direct) {
+    g.q = direct ? (const void *)grad_q_kernel<T, DP, MG, PG, SUB, true> : (const void *)grad_q_kernel<T, DP, MG, PG, SUB, false>;
+    g.q_rows = QShape<T, DP, MG, PG, SUB>::ROWS;
+    g.q_threads = QShape<T, DP, MG, PG, SUB>::THREADS;
+}
 // few: there are not enough keys for a block of the large shape on every compute unit; blocks of 32 keys then, whose waves
-// share out the queries.
-template <typename T, int DP> static GradKernels grads_for(bool direct_q, bool direct_kv, bool few) {
-    GradKernels g = {(const void *)delta_kernel<T>,
-                     direct_q ? (const void *)grad_q_kernel<T, DP, true> : (const void *)grad_q_kernel<T, DP, false>, nullptr,
-                     (const void *)join_kernel<T>, 0, 0};
-    if constexpr (sizeof(T) == 2) {
-        if (few) use_kv<T, DP, 1, 4>(g, direct_kv);
-        else use_kv<T, DP, 4, 2>(g, direct_kv);
-    } else {
-        if (few) use_kv<T, DP, 1, DP == 64 ? 4 : 2>(g, direct_kv);
-        else use_kv<T, DP, 2, 2>(g, direct_kv);
-    }
+// share out the queries.  few_q: the same of the queries.
+template <typename T, int DP> static GradKernels grads_for(bool direct_q, bool direct_kv, bool few, bool few_q) {
+    GradKernels g = {};
+    g.delta = (const void *)delta_kernel<T>;
+    g.join = (const void *)join_kernel<T>;
+    constexpr int ALL = sizeof(T) == 2 || DP == 64 ? 4 : 2;          // waves whose tiles fit into LDS
+    if (few) use_kv<T, DP, 1, ALL>(g, direct_kv);
+    else use_kv<T, DP, sizeof(T) == 2 ? 4 : 2, 2>(g, direct_kv);
+    if (few_q) use_q<T, DP, 1, ALL, 1>(g, direct_q);
+    else use_q<T, DP, 4, 1, sizeof(T) == 2 ? 2 : 1>(g, direct_q);
     return g;
 }
-template <typename T> static GradKernels grads_of(int dim, bool direct_q, bool direct_kv, bool few) {
-    return dim <= 64 ? grads_for<T, 64>(direct_q, direct_kv, few) : dim <= 96 ? grads_for<T, 96>(direct_q, direct_kv, few)
-                                                                             : grads_for<T, 128>(direct_q, direct_kv, few);
+template <typename T> static GradKernels grads_of(int dim, bool direct_q, bool direct_kv, bool few, bool few_q) {
+    return dim <= 64   ? grads_for<T, 64>(direct_q, direct_kv, few, few_q)
+           : dim <= 96 ? grads_for<T, 96>(direct_q, direct_kv, few, few_q)
+                       : grads_for<T, 128>(direct_q, direct_kv, few, few_q);
 }
 
 // Workspace: two floats a query row and head, then the first keys' parts where they are split.
@@ -541,8 +574,8 @@ static int grad_work(const spmm_attn_desc_t *a, const char *where, bool packed, 
     w->stats = (n * a->q_len * a->heads * 8 + 15) / 16 * 16;
     w->chunk = 0;
     w->part = 0;
-    const int64_t span = ((int64_t)a->window + GM + GN - 1) / GN * GN;      // queries of an ordinary block
-    if (a->window > 0 && a->window < a->k_len && a->sinks > 0 && a->sinks <= GM && a->k_len > a->sinks && a->q_len > 2 * span) {
+    const int64_t span = ((int64_t)a->window + 128 + 63) / 64 * 64;         // queries of an ordinary block of 128 keys
+    if (a->window > 0 && a->window < a->k_len && a->sinks > 0 && a->sinks <= 128 && a->k_len > a->sinks && a->q_len > 2 * span) {
         w->chunk = (int)(span < 512 ? 512 : span);
         const int64_t slots = a->batch + (packed ? a->q_len / w->chunk + a->batch : a->batch * ((a->q_len + w->chunk - 1) / w->chunk));
         w->part = slots * a->kv_heads * 2 * a->sinks * a->dim * 4;
@@ -599,12 +632,12 @@ extern "C" int spmm_attn_window_grad(const spmm_attn_desc_t *a, const spmm_attn_
     A.part = (float *)((char *)work + w.stats);
     A.chunk = w.chunk;
     int qt = 0, kt = 0, ct = 0;
-    if (a->q_len > 0 && (st = tile_count(a, W, packed, a->q_len, GM, &qt))) return st;
     const bool direct = A.k.direct && A.v.direct, direct_kv = direct && A.q.direct && A.dout.direct;
-    const bool few = (nb * a->k_len + 127) / 128 * a->kv_heads < 256;
-    const GradKernels G = a->dtype == SPMM_ATTN_F32 ? grads_of<float>(a->dim, direct, direct_kv, few)
-                          : a->dtype == SPMM_ATTN_F16 ? grads_of<_Float16>(a->dim, direct, direct_kv, few)
-                                                      : grads_of<__bf16>(a->dim, direct, direct_kv, few);
+    const bool few = (nb * a->k_len + 127) / 128 * a->kv_heads < 256, few_q = (nb * a->q_len + 127) / 128 * a->heads < 256;
+    const GradKernels G = a->dtype == SPMM_ATTN_F32 ? grads_of<float>(a->dim, direct, direct_kv, few, few_q)
+                          : a->dtype == SPMM_ATTN_F16 ? grads_of<_Float16>(a->dim, direct, direct_kv, few, few_q)
+                                                      : grads_of<__bf16>(a->dim, direct, direct_kv, few, few_q);
+    if (a->q_len > 0 && (st = tile_count(a, W, packed, a->q_len, G.q_rows, &qt))) return st;
     A.block_keys = G.keys;
     if (a->k_len > 0 && (st = tile_count(a, W, packed, a->k_len, G.keys, &kt))) return st;
     if (w.chunk && (st = tile_count(a, W, packed, a->q_len, w.chunk, &ct))) return st;
@@ -618,5 +651,5 @@ extern "C" int spmm_attn_window_grad(const spmm_attn_desc_t *a, const spmm_attn_
     if ((st = launch(G.kv, W, (kt + extra) * a->kv_heads, G.threads, args, stream))) return st;
     if (w.chunk && (st = launch(G.join, W, a->batch * a->kv_heads * A.mask.sinks, 64, args, stream))) return st;
     A.tiles = qt;
-    return launch(G.q, W, (int64_t)qt * a->heads, 256, args, stream);
+    return launch(G.q, W, (int64_t)qt * a->heads, G.q_threads, args, stream);
 }
