@@ -13,6 +13,10 @@ reference has commented out) on spmm_sddmm (spmm_pipeline.h); the final SpMM tak
 values on the device (spmm_hip_update_values_device).  Everything is stream-ordered, so one pipeline step can
 be captured in a hipGraph.
 
+``TokenPipeline`` is the same step for tokens as they come (no counterpart in the reference): projections with 4-bit
+weights (``spmm_amd.q4``), the keys and values kept in pages, and attention under a band and first columns
+(``spmm_amd.attention``) in place of SDDMM, softmax and SpMM over a CSR mask.
+
 Inputs (the reference reads three DLMC .smtx transformer weights and builds the mask with time-seeded rand(),
 sddmm_mask.h:16-80 -- neither is reproducible offline): ``dlmc_like_weight`` draws a seeded uniform-random
 pruned m x k weight (U[-1,1) values, like smtx_read's values), ``band_and_random_mask`` restates the reference's
@@ -158,3 +162,48 @@ class SparseAttentionPipeline:
         for mf in list(self.mf.values()) + [self.final]:
             mf.close()
         self.sddmm.close()
+
+
+class TokenPipeline:
+    """Q, K, V projections, cache and attention of tokens as they come, in the layout [tokens, heads, d].
+
+    w_q, w_k, w_v: ``q4.Q4Format`` of one element type with as many columns as x and heads * d, kv_heads * d and
+    kv_heads * d rows.  The cache holds ``pages`` pages of ``page_rows`` positions each; which pages a sequence has is the
+    caller's table (``attention.paged_attention``).  Every call is ordered on the device's current stream and can be
+    captured in a graph; two calls that write the same sequences' pages have to follow one another."""
+
+    def __init__(self, w_q, w_k, w_v, heads: int, kv_heads: int, pages: int, page_rows: int = 16, window: int = 0,
+                 sinks: int = 0, scale: float | None = None):
+        import torch
+        from . import attention
+        self._attention = attention
+        if heads < 1 or kv_heads < 1 or w_q.rows % heads or heads % kv_heads:
+            raise ValueError(f"{w_q.rows} rows of W_Q and {kv_heads} key heads for {heads} heads")
+        self.heads, self.kv_heads, self.dim = heads, kv_heads, w_q.rows // heads
+        if w_k.rows != kv_heads * self.dim or w_v.rows != kv_heads * self.dim:
+            raise ValueError(f"W_K and W_V need {kv_heads * self.dim} rows, they have {w_k.rows} and {w_v.rows}")
+        if not (w_q.cols == w_k.cols == w_v.cols and w_q.dtype == w_k.dtype == w_v.dtype and w_q.device == w_k.device == w_v.device):
+            raise ValueError("W_Q, W_K and W_V must agree in columns, element type and device")
+        self.w = {"Q": w_q, "K": w_k, "V": w_v}
+        self.mask = dict(window=window, sinks=sinks, scale=scale)
+        self.k_pages, self.v_pages = (torch.zeros(pages, page_rows, kv_heads, self.dim, dtype=w_q.dtype, device=w_q.device)
+                                      for _ in range(2))
+
+    def _project(self, x):
+        return (self.w[t].matvec(x).view(x.shape[0], n, self.dim) for t, n in
+                (("Q", self.heads), ("K", self.kv_heads), ("V", self.kv_heads)))
+
+    def prompt(self, x, cu, page_table, lengths):
+        """Whole sequences: x [rows, columns] with int32 offsets cu [sequences + 1] on the device; ``lengths`` int32 [sequences]
+        are those of the sequences.  Fills their pages and returns [rows, heads * d]."""
+        q, k, v = self._project(x)
+        self._attention.cache_append(k, v, self.k_pages, self.v_pages, page_table, lengths, cu=cu)
+        return self._attention.window_attention(q, k, v, cu_q=cu, **self.mask)[0].view(x.shape[0], -1)
+
+    def step(self, x, page_table, lengths, max_length: int | None = None):
+        """One new token a sequence: x [sequences, columns], ``lengths`` with the new token counted.  Adds it to the cache
+        and returns [sequences, heads * d]."""
+        q, k, v = self._project(x)
+        self._attention.cache_append(k, v, self.k_pages, self.v_pages, page_table, lengths)
+        return self._attention.paged_attention(q, self.k_pages, self.v_pages, page_table, lengths, max_length=max_length,
+                                               **self.mask)[0].view(x.shape[0], -1)

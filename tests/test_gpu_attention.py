@@ -420,3 +420,75 @@ def test_graphs(A):
             g.replay()
             torch.cuda.synchronize()
             assert all(torch.equal(a, b) for a, b in zip(res, want))
+
+
+# ------------------------------------------------------------------------------------------------ shapes of the blocks
+LARGE = [
+    # enough queries and keys for the large blocks, and the first keys' gradients split over chunks of queries
+    (2200, 2200, 16, 8, 64, 200, 4, BF16), (1300, 1700, 32, 16, 128, 130, 40, F16), (1500, 1500, 16, 16, 40, 64, 100, BF16),
+    (1200, 1200, 16, 16, 64, 100, 1, F32), (1100, 1100, 32, 32, 96, 0, 0, F16), (1030, 1030, 20, 20, 128, 70, 3, F32),
+    # few keys, first keys split
+    (2000, 2100, 4, 1, 64, 50, 33, BF16), (1000, 1000, 2, 2, 128, 100, 128, F32), (900, 900, 2, 1, 96, 60, 2, F16),
+]
+
+
+@pytest.mark.parametrize("case", LARGE, ids=str)
+def test_block_shapes(A, case):
+    nq, nk, h, hk, d, window, sinks, dtype = case
+    q, k, v = rnd(1, nq, h, d, dtype=dtype), rnd(2, nk, hk, d, dtype=dtype), rnd(3, nk, hk, d, dtype=dtype)
+    do = rnd(4, nq, h, d, dtype=dtype)
+    out, lse = A.window_attention(q[None], k[None], v[None], window, sinks)
+    got = A.window_attention_backward(do[None], q[None], k[None], v[None], out, lse, window, sinks)
+    for kv in range(0, hk, max(1, hk // 3)):                     # a few key heads and their groups in float64
+        group = slice(kv * (h // hk), (kv + 1) * (h // hk))
+        r = O.attention(q[:, group], k[:, kv:kv + 1], v[:, kv:kv + 1], window, sinks)
+        O.check("out", out[0][:, group], r["out"], r["tol_out"])
+        O.check("lse", lse[0][:, group], r["lse"], r["tol_lse"])
+        g = O.gradients(r, do[:, group])
+        O.check("dq", got[0][0][:, group], g["dq"], g["tol_dq"])
+        O.check("dk", got[1][0][:, kv:kv + 1], g["dk"], g["tol_dk"])
+        O.check("dv", got[2][0][:, kv:kv + 1], g["dv"], g["tol_dv"])
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=str)
+def test_large_packed(A, dtype):
+    """The split of the first keys in a ragged batch, with sequences shorter and longer than a chunk and rows behind."""
+    lens, h, hk, d, window, sinks = [1500, 0, 3, 640, 900], 8, 4, 64, 100, 20
+    n = sum(lens)
+    q, do = rnd(1, n + 90, h, d, dtype=dtype), rnd(4, n + 90, h, d, dtype=dtype)
+    k, v = rnd(2, n + 90, hk, d, dtype=dtype), rnd(3, n + 90, hk, d, dtype=dtype)
+    cu = torch.tensor([0] + list(itertools.accumulate(lens)), dtype=torch.int32).cuda()
+    out, lse = A.window_attention(q, k, v, window, sinks, cu_q=cu)
+    got = A.window_attention_backward(do, q, k, v, out, lse, window, sinks, cu_q=cu)
+    at = 0
+    for m in lens:
+        s = slice(at, at + m)
+        r = O.attention(q[s], k[s], v[s], window, sinks)
+        O.check("out", out[s], r["out"], r["tol_out"])
+        g = O.gradients(r, do[s])
+        for name, x in zip(("dq", "dk", "dv"), got):
+            O.check(name, x[s], g[name], g["tol_" + name])
+        at += m
+    assert all((x[at:] == 0).all() for x in (out,) + got)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("value", [math.nan, math.inf])
+def test_masked_places_do_not_leak_in_large_blocks(A, dtype, value):
+    n, h, hk, d, window, sinks, where = 1100, 32, 32, 64, 70, 2, 333
+    base = [rnd(i, 1, n, h if i in (1, 4) else hk, d, dtype=dtype) for i in (1, 2, 3, 4)]
+    seen = O.visible(n, n, window, sinks)
+    rows, keys = ~seen[:, where], ~seen[where]
+    run = lambda q, k, v, do: (lambda o, l: (o, l) + A.window_attention_backward(do, q, k, v, o, l, window, sinks))(
+        *A.window_attention(q, k, v, window, sinks))
+    ref = run(*base)
+    for i in range(4):
+        x = [t.clone() for t in base]
+        x[i][0, where, :, 3] = value
+        got = run(*x)
+        if i in (1, 2):
+            assert all(torch.equal(got[j][0][rows], ref[j][0][rows]) for j in (0, 1, 2))
+        else:
+            other = torch.arange(n) != where
+            assert all(torch.equal(got[j][0][other], ref[j][0][other]) for j in (0, 2))
+            assert all(torch.equal(got[j][0][keys], ref[j][0][keys]) for j in (3, 4))
