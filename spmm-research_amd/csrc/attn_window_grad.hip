@@ -11,7 +11,7 @@
 namespace attn {
 
 // What the two kernels below need of every query row, 16 rows x heads a block, 16 lanes a row, 8 elements a lane:
-// lse in powers of two (+inf where the query sees nothing: every weight is then exp2(x - inf) = 0), and D.
+// lse in powers of two (+inf where the query sees nothing: every weight is then exp2(x - inf) = 0), and -D.
 template <typename T> __global__ __launch_bounds__(256) void delta_kernel(WindowArgs A) {
     const bool packed = A.cu_q != nullptr;
     const int64_t rows = (packed ? 1 : A.batch) * A.q_len, x = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
@@ -29,7 +29,7 @@ template <typename T> __global__ __launch_bounds__(256) void delta_kernel(Window
     if (mine && (threadIdx.x & 15) == 0) {
         const float l = A.lse[x];
         A.stats[2 * x] = l == -INFINITY ? INFINITY : l * LOG2E;
-        A.stats[2 * x + 1] = s;
+        A.stats[2 * x + 1] = -s;
     }
 }
 
@@ -116,7 +116,9 @@ __global__ __launch_bounds__(64 * MG * PG, sizeof(T) == 2 && PG == 1 ? 2 : 1) vo
     f32x16 dq[ND];
     auto step = [&](auto careful, int j0, const T *tk, const T *tv) __attribute__((always_inline)) {
         const bool full = A.mask.all(w0, w1, j0, j0 + 31);
-        f32x16 sc = zero16(), dp = zero16();
+        f32x16 sc = zero16(), dp;                    // dP - D: the sums start from -D
+#pragma unroll
+        for (int r = 0; r < 16; ++r) dp[r] = delta;
 #pragma unroll
         for (int st = 0; st < NS; ++st) {
             sc = mma32(L::row_frag(tk, lane & 31, st * 16 + h * 8), qf[st], sc);
@@ -124,7 +126,7 @@ __global__ __launch_bounds__(64 * MG * PG, sizeof(T) == 2 && PG == 1 ? 2 : 1) vo
         }
 #pragma unroll
         for (int r = 0; r < 16; ++r)
-            sc[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[r], A.scale2, -lse2)) * (dp[r] - delta);
+            sc[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[r], A.scale2, -lse2)) * dp[r];
         if (!full) {
             asm volatile("");                        // a branch, not 16 selects in every tile
 #pragma unroll
@@ -335,11 +337,14 @@ __device__ __forceinline__ bool grad_kv_block(const WindowArgs &A, KvShared<T, D
             // the rows of this wave's queries: every wave the same number of loads
             const int n = max(0, min(rows - 32 * part, 32));
             const Buffer b(next_s + (int64_t)32 * part * A.heads * 2, n > 0 ? ((n - 1) * A.heads + 1) * 8 : 0);
-            b.to_lds4(sh.s[buf] + 64 * part, (lane >> 1) * A.heads * 8 + (lane & 1) * 4);
+            b.to_lds4(sh.s[buf] + 64 * part, (lane & 31) * A.heads * 8 + h * 4);      // 32 lse, then 32 -D
         } else {
             Move::copy(tid, A.dim, sh.q[buf], [&](int r) { return r < rows ? next_q + r * A.q.row : nullptr; });
             Move::copy(tid, A.dim, sh.d[buf], [&](int r) { return r < rows ? next_d + r * A.dout.row : nullptr; });
-            for (int e = tid; e < 2 * QN; e += THREADS) sh.s[buf][e] = e / 2 < rows ? next_s[(int64_t)(e / 2) * A.heads * 2 + e % 2] : 0.f;
+            for (int e = tid; e < 2 * QN; e += THREADS) {
+                const int r = e / 64 * 32 + e % 32;
+                sh.s[buf][e] = r < rows ? next_s[(int64_t)r * A.heads * 2 + e / 32 % 2] : 0.f;
+            }
         }
         advance();
     };
@@ -354,21 +359,29 @@ __device__ __forceinline__ bool grad_kv_block(const WindowArgs &A, KvShared<T, D
     auto last_for = [&](int a, int b) { return A.mask.window == 0 || b < A.mask.sinks ? i1 : min(i1, a + A.mask.window - 1 - shift); };
     const int all_a = max(n1 - shift, i0), all_b = last_for(n0, n1) - QN + 1;
     const int own_a = max(c1 - shift, i0), own_b = last_for(c0, c1) - 31;
+    frag<T> kf[sizeof(T) == 2 ? NS : 1];             // the wave's keys: 32-bit ones would take twice the registers
     // rows behind the last query are zeros, lse and D too: P = 1 then, and adds 1 * 0
     auto step = [&](int j0, const T *tq, const T *td, const float *ts) __attribute__((always_inline)) {
-        f32x16 sc = zero16(), dp = zero16();
+        f32x16 sc = zero16(), dp;                    // dP - D: the sums start from -D
+#pragma unroll
+        for (int r = 0; r < 16; r += 4) {
+            const f32x4 x = *reinterpret_cast<const f32x4 *>(ts + 32 + row_of(r) + 4 * h);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) dp[r + i] = x[i];
+        }
 #pragma unroll
         for (int st = 0; st < NS; ++st) {
-            sc = mma32(L::row_frag(tq, lane & 31, st * 16 + h * 8), L::row_frag(sh.k, kg * 32 + (lane & 31), st * 16 + h * 8), sc);
+            const frag<T> k = sizeof(T) == 2 ? kf[st % (sizeof(T) == 2 ? NS : 1)] : L::row_frag(sh.k, kg * 32 + (lane & 31), st * 16 + h * 8);
+            sc = mma32(L::row_frag(tq, lane & 31, st * 16 + h * 8), k, sc);
             dp = mma32(L::row_frag(td, lane & 31, st * 16 + h * 8), L::row_frag(sh.v, kg * 32 + (lane & 31), st * 16 + h * 8), dp);
         }
 #pragma unroll
-        for (int r2 = 0; r2 < 16; r2 += 2) {
-            const f32x4 st = *reinterpret_cast<const f32x4 *>(ts + 2 * (row_of(r2) + 4 * h));
+        for (int r4 = 0; r4 < 16; r4 += 4) {
+            const f32x4 l = *reinterpret_cast<const f32x4 *>(ts + row_of(r4) + 4 * h);
 #pragma unroll
-            for (int r = r2; r < r2 + 2; ++r) {
-                sc[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[r], A.scale2, -st[2 * (r - r2)]));
-                dp[r] = sc[r] * (dp[r] - st[2 * (r - r2) + 1]);
+            for (int r = r4; r < r4 + 4; ++r) {
+                sc[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[r], A.scale2, -l[r - r4]));
+                dp[r] = sc[r] * dp[r];
             }
         }
         if (j0 < own_a || j0 > own_b) {
@@ -411,6 +424,11 @@ __device__ __forceinline__ bool grad_kv_block(const WindowArgs &A, KvShared<T, D
         }
     }
     __syncthreads();
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+        for (int st = 0; st < NS; ++st) kf[st] = L::row_frag(sh.k, kg * 32 + (lane & 31), st * 16 + h * 8);
+        settled<T>(kf);
+    }
     bool fine = true;
     for (int it = 0, j0 = first_j, buf = 0; it < tiles; ++it) {
         if (AHEAD) {
@@ -525,9 +543,16 @@ template <typename T> __global__ __launch_bounds__(64) void join_kernel(WindowAr
     for (int e = threadIdx.x; e < 2 * A.dim; e += 64) {
         const int64_t x = (int64_t)(e / A.dim * A.mask.sinks + key) * A.dim + e % A.dim;       // keys' gradients, then values'
         float sum = part_of(A, b, kv)[x];
-        // the chunks that hold queries behind the window's last
-        for (int c = max(0, end + 1) / A.chunk; end + 1 < s.nq && c * (int64_t)A.chunk < s.nq; ++c)
-            sum += part_of(A, chunk_slot(A, s, packed, c), kv)[x];
+        // the chunks that hold queries behind the window's last, in order, eight on their way at a time
+        const int c0 = max(0, end + 1) / A.chunk, c1 = end + 1 < s.nq ? (s.nq - 1) / A.chunk : -1;
+        for (int c = c0; c <= c1; c += 8) {
+            float y[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) y[i] = part_of(A, chunk_slot(A, s, packed, min(c + i, c1)), kv)[x];
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (c + i <= c1) sum += y[i];
+        }
         const Rows &R = e < A.dim ? A.dk : A.dv;
         seq_base<T>(R, s, s.k0, packed, kv)[key * R.row + e % A.dim] = narrow<T>(e < A.dim ? sum * A.scale : sum);
     }
