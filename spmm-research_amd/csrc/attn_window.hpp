@@ -56,16 +56,20 @@ template <typename T> __device__ __forceinline__ frag<T> next_operand(const f32x
 template <typename T, int DP, int ROWS> struct Careful {
     f32x16 acc[DP / 32], w[ROWS / 32];
 };
-template <typename T, int DP, int ROWS>
+// BOTH: what rounding w to the type leaves enters as well, after it.
+template <typename T, int DP, int ROWS, bool BOTH = false>
 __device__ __attribute__((noinline)) void careful_product(Careful<T, DP, ROWS> *c, const T *tile, int lane, Mask mask, int p, int j0,
                                                           bool by_key, int last) {
 #pragma unroll 1
     for (int n = 0; n < ROWS / 32; ++n)
 #pragma unroll 1
         for (int k2 = 0; k2 < 2; ++k2) {
-            frag<T> pf;
+            frag<T> pf, low;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) pf[j] = narrow<T>(c->w[n][8 * k2 + j]);
+            for (int j = 0; j < 8; ++j) {
+                pf[j] = narrow<T>(c->w[n][8 * k2 + j]);
+                low[j] = narrow<T>(c->w[n][8 * k2 + j] - (float)pf[j]);
+            }
 #pragma unroll 1
             for (int d = 0; d < DP / 32; ++d) {
                 frag<T> f = Tile<T, DP>::col_frag(tile, n * 32 + k2 * 16, d * 32, lane);
@@ -73,6 +77,7 @@ __device__ __attribute__((noinline)) void careful_product(Careful<T, DP, ROWS> *
                 for (int j = 0; j < 8; ++j)
                     if (!finite_f((float)f[j])) f[j] = (T)0.f;
                 c->acc[d] = mma32(f, pf, c->acc[d]);
+                if (BOTH) c->acc[d] = mma32(f, low, c->acc[d]);
             }
         }
 #pragma unroll 1

@@ -2,9 +2,11 @@
 //
 // With P = exp(scale Q K^T - lse) on the visible places, D_i = <dO_i, O_i>, dP = dO V^T and dS = P o (dP - D):
 //   dV = P^T dO,   dK = scale dS^T Q,   dQ = scale dS K.
-// P is formed again from the saved lse instead of being kept.  Two kernels form it, one that owns keys (dK, dV: sums over
-// the queries that see them, over every query head of the group in order) and one that owns queries (dQ): seven
+// P is formed again from the saved lse instead of being kept.  Two kernels form it, one that owns queries (dQ) and one that
+// owns keys (dK, dV: sums over the queries that see them, over every query head of the group in order): seven
 // products in place of five, but each sum has one owner, so there are no atomics and no order that varies.
+// With 16-bit types P and dS are rounded to them for dV and dK.  For dQ dS goes in two 16-bit parts, and the row sum of dS,
+// which is zero but for the rounding of out in D, corrects D for dK.
 // Layouts as in the forward kernel: a product's result is the next product's operand in registers.
 #include "attn_window.hpp"
 
@@ -114,6 +116,7 @@ __global__ __launch_bounds__(64 * MG * PG, sizeof(T) == 2 && PG == 1 ? 2 : 1) vo
         if (!A.mask.all(pmin, pmax, j0, j0 + GN - 1) && Move::any_not_finite(tid, tk)) odd = 1;
     };
     f32x16 dq[ND];
+    float left;                                      // sum of the row's dS
     auto step = [&](auto careful, int j0, const T *tk, const T *tv) __attribute__((always_inline)) {
         const bool full = A.mask.all(w0, w1, j0, j0 + 31);
         f32x16 sc = zero16(), dp;                    // dP - D: the sums start from -D
@@ -134,18 +137,29 @@ __global__ __launch_bounds__(64 * MG * PG, sizeof(T) == 2 && PG == 1 ? 2 : 1) vo
                 if (!A.mask.sees(p, j0 + row_of(r) + 4 * h)) sc[r] = 0.f;
         }
         // a seen key that is not finite makes the row's weights NaN, so it need not be put back
+#pragma unroll
+        for (int r = 0; r < 16; ++r) left += sc[r];
         if constexpr (!careful) {
 #pragma unroll
             for (int k2 = 0; k2 < 2; ++k2) {
                 const frag<T> dsf = next_operand<T>(sc, k2);
+                frag<T> low = {};                    // what rounding dS to 16 bits leaves
+                if constexpr (sizeof(T) == 2) {
 #pragma unroll
-                for (int d = 0; d < ND; ++d) dq[d] = mma32(L::col_frag(tk, k2 * 16, d * 32, lane), dsf, dq[d]);
+                    for (int j = 0; j < 8; ++j) low[j] = narrow<T>(sc[8 * k2 + j] - (float)dsf[j]);
+                }
+#pragma unroll
+                for (int d = 0; d < ND; ++d) {
+                    const frag<T> kf = L::col_frag(tk, k2 * 16, d * 32, lane);
+                    dq[d] = mma32(kf, dsf, dq[d]);
+                    if constexpr (sizeof(T) == 2) dq[d] = mma32(kf, low, dq[d]);
+                }
             }
         } else {
             Careful<T, DP, 32> c;
             for (int d = 0; d < ND; ++d) c.acc[d] = dq[d];
             c.w[0] = sc;
-            careful_product<T, DP, 32>(&c, tk, lane, A.mask, p, j0, true, -1);
+            careful_product<T, DP, 32, sizeof(T) == 2>(&c, tk, lane, A.mask, p, j0, true, -1);
             for (int d = 0; d < ND; ++d) dq[d] = c.acc[d];
         }
     };
@@ -153,6 +167,7 @@ __global__ __launch_bounds__(64 * MG * PG, sizeof(T) == 2 && PG == 1 ? 2 : 1) vo
     auto run = [&](auto careful) {
 #pragma unroll
         for (int d = 0; d < ND; ++d) dq[d] = zero16();
+        left = 0.f;
         if (tiles) {
             if (DIRECT) send(tile_at(0), sk[0], sv[0]);
             settle(tile_at(0), sk[0], sv[0]);
@@ -178,6 +193,7 @@ __global__ __launch_bounds__(64 * MG * PG, sizeof(T) == 2 && PG == 1 ? 2 : 1) vo
         __syncthreads();
         run(std::true_type{});
     }
+    left += __shfl_xor(left, 32);
     if constexpr (PG > 1) {                          // the parts' sums, in order, through the tiles' place in LDS
         float *mail = reinterpret_cast<float *>(sk) + mg * ND * 16 * 64 + lane;
 #pragma unroll 1
@@ -188,6 +204,7 @@ __global__ __launch_bounds__(64 * MG * PG, sizeof(T) == 2 && PG == 1 ? 2 : 1) vo
                 for (int d = 0; d < ND; ++d)
 #pragma unroll
                     for (int r = 0; r < 16; ++r) mail[(d * 16 + r) * 64] = dq[d][r];
+                mail[ND * 16 * 64 * MG] = left;
             }
             __syncthreads();
             if (part == 0) {
@@ -195,10 +212,14 @@ __global__ __launch_bounds__(64 * MG * PG, sizeof(T) == 2 && PG == 1 ? 2 : 1) vo
                 for (int d = 0; d < ND; ++d)
 #pragma unroll
                     for (int r = 0; r < 16; ++r) dq[d][r] += mail[(d * 16 + r) * 64];
+                left += mail[ND * 16 * 64 * MG];
             }
         }
     }
     if (!mine || part != 0) return;
+    // A row of dS sums to zero; what is left is by how much D, taken from the rounded out, is off.  The kernel that owns keys
+    // runs next and gets it right.
+    if (h == 0) A.stats[2 * ((packed ? s.q0 + i : s.b * A.q_len + i) * A.heads + head) + 1] -= left;
     T *dst = seq_base<T>(A.dq, s, s.q0, packed, head) + i * A.dq.row;
 #pragma unroll
     for (int d = 0; d < ND; ++d)
@@ -671,10 +692,10 @@ extern "C" int spmm_attn_window_grad(const spmm_attn_desc_t *a, const spmm_attn_
     void *args[] = {&A};
     const int64_t rows = nb * a->q_len * a->heads;
     if ((st = launch(G.delta, W, (rows + 15) / 16, 256, args, stream))) return st;
+    A.tiles = qt;
+    if ((st = launch(G.q, W, (int64_t)qt * a->heads, G.q_threads, args, stream))) return st;
     A.tiles = kt;
     const int64_t extra = w.chunk ? (int64_t)ct * ((A.mask.sinks + G.keys - 1) / G.keys) : 0;
     if ((st = launch(G.kv, W, (kt + extra) * a->kv_heads, G.threads, args, stream))) return st;
-    if (w.chunk && (st = launch(G.join, W, a->batch * a->kv_heads * A.mask.sinks, 64, args, stream))) return st;
-    A.tiles = qt;
-    return launch(G.q, W, (int64_t)qt * a->heads, G.q_threads, args, stream);
+    return w.chunk ? launch(G.join, W, a->batch * a->kv_heads * A.mask.sinks, 64, args, stream) : SPMM_HIP_OK;
 }
