@@ -5,11 +5,10 @@
 // kernel and it is laid out for loads that go straight into the matrix instructions, with no LDS on the way:
 //  - a wave takes 16 keys at a time; S^T = K Q^T (16 keys x up to 16 heads) has a lane's 16-byte piece of one key's row
 //    as its first operand;
-//  - S^T leaves a lane with keys 4 (l / 16) + r, r = 0..3, of head l % 16.  exp(S^T) register r is then, as it stands, the
-//    first operand of a 16x16x4 product in 32-bit floats over the keys {r, 4 + r, 8 + r, 12 + r}, whose second operand is
-//    value row 4 (l / 16) + r: lane l % 16 loads 16 bytes of that row and gives one element to each of 8 products.
-//    The 32-bit instruction costs 8 times a 16-bit one and is still under the time of the loads; in return the
-//    weights are not rounded and the values need no transposition.
+//  - S^T leaves a lane with keys 4 (l / 16) + r, r = 0..3, of head l % 16.  exp(S^T) is then, as it stands, the first
+//    operand of a 16x16x16 product (of four 16x16x4 ones in 32 bits), whose second operand is element j of value rows
+//    4 (l / 16) + 0..3: lane l % 16 loads a piece of those four rows, and element j of each makes up product j.  The
+//    values need no transposition.  16-bit products take the weights in two parts, so they lose nothing by rounding.
 // A block's four waves share a stretch of the keys and join through LDS; when there are few sequences the keys are
 // split over several blocks, and a second kernel joins their parts in order.
 #include "attn_common.hpp"
@@ -46,6 +45,16 @@ __device__ __forceinline__ Span span_of(int len, int window, int sinks) {
     return s;
 }
 
+// Depth 16: lane l gives row (column) l % 16 at depths 4 (l / 16) + 0..3.
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ f32x4 mma16x16(bf16x4 a, bf16x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(i16x4, a), __builtin_bit_cast(i16x4, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mma16x16(f16x4 a, f16x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x16f16(a, b, c, 0, 0, 0);
+}
+
 __device__ __align__(16) const float zero_row[SPMM_ATTN_MAX_DIM] = {};
 
 // E elements of a row from element e on, zero beyond dim; `row` is zero_row where there is none.
@@ -59,6 +68,31 @@ template <typename T, int E> struct Piece {
         return v;
     }
 };
+
+// o[j] += weights (16 heads x 16 keys, as the scores' product leaves them) x column j of the lanes' pieces of the values.
+template <typename T, int VE>
+__device__ __forceinline__ void add_values(f32x4 (&o)[VE], const f32x4 &w, const typename Piece<T, VE>::vec (&v)[4]) {
+    if constexpr (sizeof(T) == 2) {
+        typedef T t4 __attribute__((ext_vector_type(4)));
+        t4 hi, lo;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            hi[r] = narrow<T>(w[r]);
+            lo[r] = narrow<T>(w[r] - (float)hi[r]);
+        }
+#pragma unroll
+        for (int j = 0; j < VE; ++j) {
+            const t4 b = {v[0][j], v[1][j], v[2][j], v[3][j]};
+            o[j] = mma16x16(hi, b, o[j]);
+            o[j] = mma16x16(lo, b, o[j]);
+        }
+    } else {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int j = 0; j < VE; ++j) o[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(w[r], v[r][j], o[j], 0, 0, 0);
+    }
+}
 
 template <typename T, int DP>
 __global__ __launch_bounds__(PW * 64, sizeof(T) == 2 ? 4 : 2) void paged_kernel(PagedArgs A) {
@@ -152,11 +186,7 @@ __global__ __launch_bounds__(PW * 64, sizeof(T) == 2 ? 4 : 2) void paged_kernel(
             sc[r] = __builtin_amdgcn_exp2f(sc[r] - base);
             sum += sc[r];
         }
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-#pragma unroll
-            for (int j = 0; j < VE; ++j)
-                o[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(sc[r], (float)vr[r][j], o[j], 0, 0, 0);
+        add_values<T, VE>(o, sc, vr);
     }
     sum += __shfl_xor(sum, 16);
     sum += __shfl_xor(sum, 32);

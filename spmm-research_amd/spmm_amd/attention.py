@@ -141,10 +141,12 @@ def _window_operands(q, k, v, window, sinks, scale, cu_q, cu_k, zero_rest):
     if packed:
         cu_k = cu_q if cu_k is None else cu_k
         _tensor("cu_q", cu_q, torch.int32, dev, None, True)
-        _tensor("cu_k", cu_k, torch.int32, dev, None, True)
-        if cu_q.ndim != 1 or cu_q.shape != cu_k.shape or len(cu_q) < 1:
+        if cu_k is not cu_q:
+            _tensor("cu_k", cu_k, torch.int32, dev, None, True)
+        size = cu_q.shape
+        if len(size) != 1 or size[0] < 1 or size != cu_k.shape:
             raise ValueError("cu_q and cu_k must be vectors of the number of sequences + 1")
-        batch, pq, pk = len(cu_q) - 1, cu_q.data_ptr(), cu_k.data_ptr()
+        batch, pq, pk = size[0] - 1, cu_q.data_ptr(), cu_k.data_ptr()
     d = _desc(q, dev, kd[-2], window, sinks, scale, batch, qd[-3], kd[-3], zero_rest and packed)
     return packed, d, pq, pk, _rows(q, qs, packed), _rows(k, ks, packed), _rows(v, vs, packed), dev, dt
 
@@ -162,12 +164,12 @@ def window_attention(q, k, v, window: int = 0, sinks: int = 0, scale: float | No
     st, where = _place(dev, stream)
     with where or _HERE:
         if out is None:
-            out = torch.empty(q.shape, dtype=dt, device=q.device)
+            out = q.new_empty(q.shape)
             os = out.stride()
         else:
             os = _tensor("out", out, dt, dev, q.shape)
         if lse is None:
-            lse = torch.empty(q.shape[:-1], dtype=torch.float32, device=q.device)
+            lse = q.new_empty(q.shape[:-1], dtype=torch.float32)
         else:
             _tensor("lse", lse, torch.float32, dev, q.shape[:-1], True)
         if packed and d.batch == 0 and d.zero_rest:
@@ -193,13 +195,13 @@ def window_attention_backward(dout, q, k, v, out, lse, window: int = 0, sinks: i
         res, rows = [], []
         for name, g, t in (("dq", dq, q), ("dk", dk, k), ("dv", dv, v)):
             if g is None:
-                g = torch.empty(t.shape, dtype=dt, device=t.device)
+                g = t.new_empty(t.shape)
                 s = g.stride()
             else:
                 s = _tensor(name, g, dt, dev, t.shape)
             res.append(g)
             rows.append(_rows(g, s, packed))
-        work = torch.empty(need.value, dtype=torch.uint8, device=q.device)
+        work = q.new_empty(need.value, dtype=torch.uint8)
         if packed and d.batch == 0 and d.zero_rest:
             return tuple(g.zero_() for g in res)
     _check("window_attention_backward", lib.spmm_attn_window_grad(d, dr, qr, kr, vr, outr, lse.data_ptr(), pq, pk, *rows,
@@ -246,15 +248,15 @@ def paged_attention(q, k_pages, v_pages, page_table, lengths, window: int = 0, s
     _check("paged_attention", lib.spmm_attn_paged_work(d, longest, need))
     with where or _HERE:
         if out is None:
-            out = torch.empty(q.shape, dtype=dt, device=q.device)
+            out = q.new_empty(q.shape)
             os = out.stride()
         else:
             os = _tensor("out", out, dt, dev, q.shape)
         if lse is None:
-            lse = torch.empty(q.shape[:-1], dtype=torch.float32, device=q.device)
+            lse = q.new_empty(q.shape[:-1], dtype=torch.float32)
         else:
             _tensor("lse", lse, torch.float32, dev, q.shape[:-1], True)
-        work = torch.empty(need.value, dtype=torch.uint8, device=q.device) if need.value else None
+        work = q.new_empty(need.value, dtype=torch.uint8) if need.value else None
     _check("paged_attention", lib.spmm_attn_paged(
         d, _Rows(q.data_ptr(), qs[0], 0, qs[1]), pages, longest, _Rows(out.data_ptr(), os[0], 0, os[1]), lse.data_ptr(),
         work.data_ptr() if work is not None else None, need.value, st))
@@ -275,9 +277,9 @@ def cache_append(k, v, k_pages, v_pages, page_table, lengths, cu=None, stream: i
     batch, pc = rows, None
     if cu is not None:
         _tensor("cu", cu, torch.int32, dev, None, True)
-        if cu.ndim != 1 or len(cu) < 1:
+        if cu.ndim != 1 or cu.shape[0] < 1:
             raise ValueError("cu must be a vector of the number of sequences + 1")
-        batch, pc = len(cu) - 1, cu.data_ptr()
+        batch, pc = cu.shape[0] - 1, cu.data_ptr()
     pages = _pages(k_pages, v_pages, page_table, lengths, dim, dt, dev, batch)
     if k_pages.shape[2] != heads:
         raise ValueError(f"{heads} key heads, the pages have {k_pages.shape[2]}")

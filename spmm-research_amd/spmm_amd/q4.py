@@ -90,7 +90,7 @@ class Q4Format:
         st, where = _place(self._dev, stream)
         with where or _HERE:
             if out is None:
-                out = torch.empty(shape, dtype=self.dtype, device=self.device)
+                out = x.new_empty(shape)
                 os = out.stride()
             else:
                 os = _tensor("out", out, self.dtype, self._dev, shape)
