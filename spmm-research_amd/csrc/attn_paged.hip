@@ -17,7 +17,11 @@ namespace attn {
 
 constexpr int PW = 4;                        // waves of a block
 constexpr int PK = 16;                       // keys a wave takes at a time
-constexpr int SPLIT_MIN = 256;               // keys a block takes at least
+constexpr int ALONE = 256;                   // keys up to which a block takes a sequence alone
+constexpr int SPLIT_MIN = 64;                // keys a block takes at least otherwise: one tile a wave
+constexpr int SPLIT_MAX = 256;               // parts of a sequence at most
+// blocks that a compute unit holds at once
+__host__ __device__ constexpr int paged_blocks(bool half) { return half ? 4 : 2; }
 
 struct PagedArgs {
     Rows q, out;
@@ -95,7 +99,7 @@ __device__ __forceinline__ void add_values(f32x4 (&o)[VE], const f32x4 &w, const
 }
 
 template <typename T, int DP>
-__global__ __launch_bounds__(PW * 64, sizeof(T) == 2 ? 4 : 2) void paged_kernel(PagedArgs A) {
+__global__ __launch_bounds__(PW * 64, paged_blocks(sizeof(T) == 2)) void paged_kernel(PagedArgs A) {
     // a lane's columns of the values: VE from VE (lane % 16) on
     constexpr int NS = DP / 32, VE = DP / 16;
     const int group = A.heads / A.kv_heads, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, h4 = lane >> 4;
@@ -233,10 +237,12 @@ __global__ __launch_bounds__(PW * 64, sizeof(T) == 2 ? 4 : 2) void paged_kernel(
     }
 }
 
-// One wave a (sequence, head): its parts joined in an order that is fixed by their number.
-template <typename T> __global__ __launch_bounds__(64) void paged_join_kernel(PagedArgs A) {
+// A block a (sequence, head): its parts joined in an order that is fixed by their number.  Each of the four waves takes a
+// quarter of them, eight parts on their way at a time.
+constexpr int JW = 4;
+template <typename T> __global__ __launch_bounds__(JW * 64) void paged_join_kernel(PagedArgs A) {
     const int64_t x = blockIdx.x, b = x / A.heads;
-    const int hd = (int)(x % A.heads), lane = threadIdx.x, w = A.dim + 2;
+    const int hd = (int)(x % A.heads), lane = threadIdx.x & 63, wave = threadIdx.x >> 6, w = A.dim + 2;
     const float *p = A.part + x * A.splits * w;
     float mx = -INFINITY;
     for (int s = lane; s < A.splits; s += WAVE) mx = fmaxf(mx, p[(int64_t)s * w]);
@@ -245,8 +251,9 @@ template <typename T> __global__ __launch_bounds__(64) void paged_join_kernel(Pa
     const float base = mx == -INFINITY ? 0.f : mx;
     float tot = 0.f, a0 = 0.f, a1 = 0.f;
     const int e0 = min(lane, A.dim - 1), e1 = min(lane + WAVE, A.dim - 1);
-    for (int s0 = 0; s0 < A.splits; s0 += WAVE) {
-        const int n = min(WAVE, A.splits - s0);
+    const int per = (A.splits + JW - 1) / JW, last = min((wave + 1) * per, A.splits);
+    for (int s0 = wave * per; s0 < last; s0 += WAVE) {
+        const int n = min(WAVE, last - s0);
         const float *ps = p + (int64_t)s0 * w;
         float f = 0.f, add = 0.f;
         if (lane < n) {
@@ -265,6 +272,18 @@ template <typename T> __global__ __launch_bounds__(64) void paged_join_kernel(Pa
                 a1 += fs * pi[e1];
             }
         }
+    }
+    __shared__ float st[JW], s0[JW][WAVE], s1[JW][WAVE];
+    if (lane == 0) st[wave] = tot;
+    s0[wave][lane] = a0;
+    s1[wave][lane] = a1;
+    __syncthreads();
+    if (wave) return;
+#pragma unroll
+    for (int i = 1; i < JW; ++i) {
+        tot += st[i];
+        a0 += s0[i][lane];
+        a1 += s1[i][lane];
     }
     const float inv = tot == 0.f ? 0.f : 1.f / tot;
     T *dst = (T *)A.out.ptr + b * A.out.seq + hd * A.out.head;
@@ -304,7 +323,7 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs A) {
     } else {
         pos = (int64_t)A.lengths[b] - 1;
     }
-    if (pos < 0 || A.lengths[b] > A.table_cols * A.page_rows) return;
+    if (pos < 0 || (A.lengths[b] - 1) / A.page_rows >= A.table_cols) return;
     const int64_t pg = A.table[b * A.table_stride + pos / A.page_rows];
     if (pg < 0 || pg >= A.pages) return;
     const int64_t slot = pos % A.page_rows;
@@ -351,14 +370,19 @@ static int check_pages(const spmm_attn_desc_t *a, const spmm_attn_pages_t *p, co
     return SPMM_HIP_OK;
 }
 
-// Blocks that share a sequence's keys: enough for eight blocks a compute unit in all, each with SPLIT_MIN keys or more.
+// Blocks that share a sequence's keys: as many as are on the compute units at once (four each, two with 32-bit elements), each
+// with SPLIT_MIN keys or more, SPLIT_MAX parts at most; none share up to ALONE keys, where a second launch costs more.
+// In bf16, 8 heads over 1 of 128: 1000 keys 9.8 us (parts of 128 keys 11.2, of 256 14.2, of 512 20.2), 8192 keys 11.7 (20.5 with
+// 512); 2 key heads, 100000 keys 30.5 us with 256 parts (35 with 128 or 512).  Batch of 32 of 4096 keys, 32 heads over 8:
+// 1024 blocks 108 us, 512 blocks 115, 2048 blocks 111; in 32 bits 512 blocks 250, 256 blocks 390.
 static int64_t split_count(const spmm_attn_desc_t *a, int64_t max_length) {
     const int64_t group = a->heads / a->kv_heads, base = a->batch * a->kv_heads * ((group + 15) / 16);
     int64_t keys = max_length;
     if (a->window && a->window < keys) keys = (int64_t)a->window + (a->sinks < keys - a->window ? a->sinks : keys - a->window);
-    const int64_t most = (keys + SPLIT_MIN - 1) / SPLIT_MIN, want = base > 0 ? (2048 + base - 1) / base : 1;
-    const int64_t n = want < most ? want : most;
-    return n < 1 ? 1 : n;
+    const int64_t most = (keys + SPLIT_MIN - 1) / SPLIT_MIN, want = base > 0 ? 256 * paged_blocks(a->dtype != SPMM_ATTN_F32) / base : 1;
+    int64_t n = want < most ? want : most;
+    n = n < SPLIT_MAX ? n : SPLIT_MAX;
+    return n < 1 || keys <= ALONE ? 1 : n;
 }
 
 template <typename T> static const void *paged_of(int dim) {
@@ -435,7 +459,7 @@ extern "C" int spmm_attn_paged(const spmm_attn_desc_t *a, const spmm_attn_rows_t
     void *args[] = {&A};
     const int64_t hb = (a->heads / a->kv_heads + 15) / 16;
     if ((st = launch(kern, W, a->batch * A.splits * hb * a->kv_heads, PW * 64, args, stream))) return st;
-    return A.splits > 1 ? launch(join, W, a->batch * a->heads, 64, args, stream) : SPMM_HIP_OK;
+    return A.splits > 1 ? launch(join, W, a->batch * a->heads, JW * 64, args, stream) : SPMM_HIP_OK;
 }
 
 extern "C" int spmm_attn_append(const spmm_attn_desc_t *a, const spmm_attn_rows_t *k, const spmm_attn_rows_t *v,
