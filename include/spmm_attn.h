@@ -14,13 +14,15 @@
  * does not see, infinities and NaN included, does not reach its results.
  *
  * Query head h reads key/value head h / (heads / kv_heads).  Element types: SPMM_ATTN_F32, SPMM_ATTN_F16,
- * SPMM_ATTN_BF16; scores, softmax statistics and sums are 32-bit floats.  With the 16-bit types the weights (and, in the
- * backward pass, their gradients) are rounded to that type before they enter a matrix product.  Results do not depend
- * on anything but the arguments: no atomics, fixed orders of summation.
+ * SPMM_ATTN_BF16; scores, softmax statistics and sums are 32-bit floats.  With the 16-bit types spmm_attn_window rounds
+ * the weights to that type before they enter a product, and spmm_attn_window_grad the weights and their gradients where
+ * they enter dv and dk; in dq and in spmm_attn_paged they enter as a rounded value plus its rounded remainder.  Results
+ * do not depend on anything but the arguments: no atomics, fixed orders of summation.
  *
- * Every pointer is a device address on `device`, calls are ordered on `stream` (a hipStream_t, NULL = the null
- * stream), hold no state between calls and can be captured in a graph.  Calls that run at the same time need separate
- * workspaces.  The current device is put back before a call returns.  Status codes are the engine's (spmm_hip.h).
+ * Every pointer is a device address on `device`, and what a call writes does not overlap what it reads.  Calls are
+ * ordered on `stream` (a hipStream_t, NULL = the null stream), hold no state between calls and can be captured in a
+ * graph.  Calls that run at the same time need separate workspaces.  The current device is put back before a call
+ * returns.  Status codes are the engine's (spmm_hip.h).
  */
 #ifndef SPMM_ATTN_H
 #define SPMM_ATTN_H

@@ -23,7 +23,7 @@ __global__ __launch_bounds__(64 * MG * PG, sizeof(T) == 2 && PG == 1 ? 2 : 1) vo
     constexpr int BM = S::ROWS, BN = S::BN, THREADS = S::THREADS, ND = DP / 32, NS = DP / 16, NK = SUB;
     __shared__ __align__(16) T sk[2][BN * L::PITCH], sv[2][BN * L::PITCH];
     __shared__ float sm[PG > 1 ? PG * MG * 32 : 1];  // the parts' maxima
-    __shared__ int odd;                              // some staged value of a partly visible tile was not finite
+    __shared__ int odd[2];                           // a value of the partly seen tile in this pair is not finite
 
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), h = lane >> 5;
     const int mg = wave % MG, part = wave / MG;      // the wave's queries, and which keys of a tile
@@ -42,7 +42,7 @@ __global__ __launch_bounds__(64 * MG * PG, sizeof(T) == 2 && PG == 1 ? 2 : 1) vo
         }
         return;
     }
-    if (tid == 0) odd = 0;
+    if (tid == 0) odd[0] = odd[1] = 0;
 
     const int shift = s.nk - s.nq, m0 = s.tile * BM, m1 = min(m0 + BM, s.nq) - 1;
     const int pmin = m0 + shift, pmax = m1 + shift;                       // positions of the block's queries
@@ -81,7 +81,7 @@ __global__ __launch_bounds__(64 * MG * PG, sizeof(T) == 2 && PG == 1 ? 2 : 1) vo
         mv.send(wave, tv, vb + (int64_t)j0 * A.v.row, A.v.row, pmax + 1 - j0, A.dim);
     };
     // the tile is in LDS but for a barrier
-    auto settle = [&](int j0, T *tk, T *tv) {
+    auto settle = [&](int j0, int buf, T *tk, T *tv) {
         if constexpr (DIRECT) {
             arrived();
         } else {
@@ -91,7 +91,7 @@ __global__ __launch_bounds__(64 * MG * PG, sizeof(T) == 2 && PG == 1 ? 2 : 1) vo
             copy(tk, kb, A.k.row);
             copy(tv, vb, A.v.row);
         }
-        if (!A.mask.all(pmin, pmax, j0, j0 + BN - 1) && Move::any_not_finite(tid, tv)) odd = 1;
+        if (!A.mask.all(pmin, pmax, j0, j0 + BN - 1) && Move::any_not_finite(tid, tv)) odd[buf] = 1;
     };
 
     f32x16 o[ND];
@@ -169,16 +169,17 @@ __global__ __launch_bounds__(64 * MG * PG, sizeof(T) == 2 && PG == 1 ? 2 : 1) vo
         for (int d = 0; d < ND; ++d) o[d] = zero16();
         if (tiles) {
             if (DIRECT) send(tile_at(0), sk[0], sv[0]);
-            settle(tile_at(0), sk[0], sv[0]);
+            settle(tile_at(0), 0, sk[0], sv[0]);
         }
         __syncthreads();
         for (int it = 0; it < tiles; ++it) {         // a tile's loads are under way while the one before it is used
             const int buf = it & 1, j0 = tile_at(it);
-            if (!careful && !A.mask.all(pmin, pmax, j0, j0 + BN - 1) && uniform(odd)) return false;
+            // The whole block leaves at the same tile: what a wave ahead finds in the next one goes to the other flag.
+            if (!careful && !A.mask.all(pmin, pmax, j0, j0 + BN - 1) && uniform(odd[buf])) return false;
             const bool more = it + 1 < tiles;
             if (DIRECT && more) send(tile_at(it + 1), sk[buf ^ 1], sv[buf ^ 1]);
             step(careful, j0 + 32 * SUB * part, sk[buf] + 32 * SUB * part * L::PITCH, sv[buf] + 32 * SUB * part * L::PITCH);
-            if (more) settle(tile_at(it + 1), sk[buf ^ 1], sv[buf ^ 1]);
+            if (more) settle(tile_at(it + 1), buf ^ 1, sk[buf ^ 1], sv[buf ^ 1]);
             __syncthreads();
         }
         return true;
@@ -280,8 +281,9 @@ template <typename T, int DP> static WindowKernel window_for(bool direct, bool f
     if constexpr (sizeof(T) == 2) return few ? window_with<T, DP, 1, 4, 1>(direct) : window_with<T, DP, 4, 1, 2>(direct);
     else return few ? window_with<T, DP, 1, DP == 64 ? 4 : 2, 1>(direct) : window_with<T, DP, 4, 1, 1>(direct);
 }
-// few: there are not enough queries for a block of the large shape on every compute unit; blocks of 32 queries then, whose
-// waves share out the keys.
+// few: blocks of the large shape would not fill half of the compute units; blocks of 32 queries then, whose waves share out
+// the keys.  512 tokens, 8 heads of 128 in bf16 (32 large blocks): 15.0 us with small blocks, 19.6 with large ones; 2048
+// tokens (128): 43.6 and 37.8, 8192 tokens: 186 and 55.  In 32 bits 50 and 89, 198 and 196, 824 and 397.
 template <typename T> static WindowKernel window_of(int dim, bool direct, bool few) {
     return dim <= 64 ? window_for<T, 64>(direct, few) : dim <= 96 ? window_for<T, 96>(direct, few) : window_for<T, 128>(direct, few);
 }
@@ -308,7 +310,7 @@ extern "C" int spmm_attn_window(const spmm_attn_desc_t *a, const spmm_attn_rows_
     if (nb == 0 || a->q_len == 0 || a->batch == 0) return SPMM_HIP_OK;
     if (!lse || (uintptr_t)lse % 4) return fail(SPMM_HIP_ERR_ARG, "%s: lse is NULL or not aligned", W);
     A.lse = lse;
-    const bool direct = A.k.direct && A.v.direct, few = (nb * a->q_len + 127) / 128 * a->heads < 256;
+    const bool direct = A.k.direct && A.v.direct, few = (nb * a->q_len + 127) / 128 * a->heads < 128;
     const WindowKernel K = a->dtype == SPMM_ATTN_F32 ? window_of<float>(a->dim, direct, few)
                            : a->dtype == SPMM_ATTN_F16 ? window_of<_Float16>(a->dim, direct, few) : window_of<__bf16>(a->dim, direct, few);
     if ((st = tile_count(a, W, packed, a->q_len, K.rows, &A.tiles))) return st;

@@ -47,7 +47,7 @@ __global__ __launch_bounds__(64 * MG * PG, sizeof(T) == 2 && PG == 1 ? 2 : 1) vo
     using S = QShape<T, DP, MG, PG, SUB>;
     constexpr int GM = S::ROWS, GN = S::KN, THREADS = S::THREADS, ND = DP / 32, NS = DP / 16;
     __shared__ __align__(16) T sk[2][GN * L::PITCH], sv[2][GN * L::PITCH];
-    __shared__ int odd;
+    __shared__ int odd[2];
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), h = lane >> 5;
     const int mg = wave % MG, part = wave / MG;      // the wave's queries, and which keys of a tile
     int kv, g, t;
@@ -61,7 +61,7 @@ __global__ __launch_bounds__(64 * MG * PG, sizeof(T) == 2 && PG == 1 ? 2 : 1) vo
             zero_rows<T>(A.dq, s.rest + (int64_t)(t - s.nq) * GM, (int64_t)(A.tiles - s.nq) * GM, GM, A.q_len, head, A.dim);
         return;
     }
-    if (tid == 0) odd = 0;
+    if (tid == 0) odd[0] = odd[1] = 0;
     const int shift = s.nk - s.nq, m0 = s.tile * GM, m1 = min(m0 + GM, s.nq) - 1;
     const int pmin = m0 + shift, pmax = m1 + shift;
     const int lo = A.mask.window ? max(0, pmin - A.mask.window + 1) : 0;
@@ -103,7 +103,7 @@ __global__ __launch_bounds__(64 * MG * PG, sizeof(T) == 2 && PG == 1 ? 2 : 1) vo
         mk.send(wave, tk, kb + (int64_t)j0 * A.k.row, A.k.row, pmax + 1 - j0, A.dim);
         mv.send(wave, tv, vb + (int64_t)j0 * A.v.row, A.v.row, pmax + 1 - j0, A.dim);
     };
-    auto settle = [&](int j0, T *tk, T *tv) {
+    auto settle = [&](int j0, int buf, T *tk, T *tv) {
         if constexpr (DIRECT) {
             arrived();
         } else {
@@ -113,7 +113,7 @@ __global__ __launch_bounds__(64 * MG * PG, sizeof(T) == 2 && PG == 1 ? 2 : 1) vo
             copy(tk, kb, A.k.row);
             copy(tv, vb, A.v.row);
         }
-        if (!A.mask.all(pmin, pmax, j0, j0 + GN - 1) && Move::any_not_finite(tid, tk)) odd = 1;
+        if (!A.mask.all(pmin, pmax, j0, j0 + GN - 1) && Move::any_not_finite(tid, tk)) odd[buf] = 1;
     };
     f32x16 dq[ND];
     float left;                                      // sum of the row's dS
@@ -170,12 +170,12 @@ __global__ __launch_bounds__(64 * MG * PG, sizeof(T) == 2 && PG == 1 ? 2 : 1) vo
         left = 0.f;
         if (tiles) {
             if (DIRECT) send(tile_at(0), sk[0], sv[0]);
-            settle(tile_at(0), sk[0], sv[0]);
+            settle(tile_at(0), 0, sk[0], sv[0]);
         }
         __syncthreads();
         for (int it = 0; it < tiles; ++it) {
             const int buf = it & 1, j0 = tile_at(it);
-            if (!careful && !A.mask.all(pmin, pmax, j0, j0 + GN - 1) && uniform(odd)) return false;
+            if (!careful && !A.mask.all(pmin, pmax, j0, j0 + GN - 1) && uniform(odd[buf])) return false;
             const bool more = it + 1 < tiles;
             if (DIRECT && more) send(tile_at(it + 1), sk[buf ^ 1], sv[buf ^ 1]);
 #pragma unroll
@@ -183,7 +183,7 @@ __global__ __launch_bounds__(64 * MG * PG, sizeof(T) == 2 && PG == 1 ? 2 : 1) vo
                 const int r = 32 * (SUB * part + u);
                 step(careful, j0 + r, sk[buf] + r * L::PITCH, sv[buf] + r * L::PITCH);
             }
-            if (more) settle(tile_at(it + 1), sk[buf ^ 1], sv[buf ^ 1]);
+            if (more) settle(tile_at(it + 1), buf ^ 1, sk[buf ^ 1], sv[buf ^ 1]);
             __syncthreads();
         }
         return true;
@@ -241,7 +241,7 @@ __device__ __forceinline__ int64_t chunk_slot(const WindowArgs &A, const Seq &s,
 }
 // last query that sees one of the keys n0 .. n1 through the window
 __device__ __forceinline__ int window_end(const WindowArgs &A, const Seq &s, int n1) {
-    return min(s.nq - 1, n1 + A.mask.window - 1 - (s.nk - s.nq));
+    return (int)min((int64_t)s.nq - 1, (int64_t)n1 + A.mask.window - 1 - (s.nk - s.nq));
 }
 
 // How a block of the kernel below is made up: KG groups of 32 keys, whose keys and values stay in LDS, times PG waves that
@@ -260,7 +260,7 @@ template <typename T, int DP, int KG, int PG> struct KvShared {
     __align__(16) T k[S::KEYS * P], v[S::KEYS * P];                  // at the end: a wave's sums for another
     __align__(16) T q[S::STAGES][S::QN * P], d[S::STAGES][S::QN * P];
     __align__(16) float s[S::STAGES][2 * S::QN];                     // lse and D of the tile's rows
-    int odd;
+    int odd[2];                                                      // a value of tile 0, 2, .. or 1, 3, .. is not finite
 };
 
 // False, with nothing written, if a value in a partly seen tile is not finite and CAREFUL does not allow for that.
@@ -292,7 +292,7 @@ __device__ __forceinline__ bool grad_kv_block(const WindowArgs &A, KvShared<T, D
         }
         return true;
     }
-    if (tid == 0) sh.odd = 0;
+    if (tid == 0) sh.odd[0] = sh.odd[1] = 0;
     const int group = A.heads / A.kv_heads;
     const int shift = s.nk - s.nq, n0 = (extra ? e0 : s.tile) * KEYS;
     const int n1 = min(n0 + KEYS, extra ? min(A.mask.sinks, s.nk) : s.nk) - 1;
@@ -459,9 +459,10 @@ __device__ __forceinline__ bool grad_kv_block(const WindowArgs &A, KvShared<T, D
             if (DIRECT) arrived();
         }
         const bool whole = j0 >= all_a && j0 <= all_b;
-        if (!whole && (Move::any_not_finite(tid, sh.q[buf]) || Move::any_not_finite(tid, sh.d[buf]))) sh.odd = 1;
+        if (!whole && (Move::any_not_finite(tid, sh.q[buf]) || Move::any_not_finite(tid, sh.d[buf]))) sh.odd[it & 1] = 1;
         __syncthreads();                             // tile `it` is there for all, and tile `it` - 1 is read
-        if (!CAREFUL && !whole && uniform(sh.odd)) {  // the whole block leaves at the same tile
+        // the whole block leaves at the same tile: what a wave ahead finds in the next one goes to the other flag
+        if (!CAREFUL && !whole && uniform(sh.odd[it & 1])) {
             fine = false;
             break;
         }
@@ -593,15 +594,21 @@ template <typename T, int DP, int MG, int PG, int SUB> static void use_q(GradKer
     g.q_rows = QShape<T, DP, MG, PG, SUB>::ROWS;
     g.q_threads = QShape<T, DP, MG, PG, SUB>::THREADS;
 }
-// few: there are not enough keys for a block of the large shape on every compute unit; blocks of 32 keys then, whose waves
-// share out the queries.  few_q: the same of the queries.
+// few: there are not enough keys to keep the compute units busy with blocks of the large shape; blocks of 32 keys then, whose
+// waves share out the queries.  few_q: the same of the queries.  Step of 512 tokens, 8 heads over 2 of 128 in bf16, with
+// blocks of 32 keys 67 us, of 128 keys 95; of 8192 tokens 324 and 254.  32-bit tiles of 128 leave no room for a fourth wave,
+// and the small shape is then never faster (2048 tokens: 1135 and 1071 us); of 64 it is (1024 tokens, 8 heads: 107 and 142).
 template <typename T, int DP> static GradKernels grads_for(bool direct_q, bool direct_kv, bool few, bool few_q) {
     GradKernels g = {};
     g.delta = (const void *)delta_kernel<T>;
     g.join = (const void *)join_kernel<T>;
     constexpr int ALL = sizeof(T) == 2 || DP == 64 ? 4 : 2;          // waves whose tiles fit into LDS
-    if (few) use_kv<T, DP, 1, ALL>(g, direct_kv);
-    else use_kv<T, DP, sizeof(T) == 2 ? 4 : 2, 2>(g, direct_kv);
+    if constexpr (ALL == 4) {
+        if (few) use_kv<T, DP, 1, 4>(g, direct_kv);
+        else use_kv<T, DP, sizeof(T) == 2 ? 4 : 2, 2>(g, direct_kv);
+    } else {
+        use_kv<T, DP, 2, 2>(g, direct_kv);
+    }
     if (few_q) use_q<T, DP, 1, ALL, 1>(g, direct_q);
     else use_q<T, DP, 4, 1, sizeof(T) == 2 ? 2 : 1>(g, direct_q);
     return g;
@@ -612,6 +619,9 @@ template <typename T> static GradKernels grads_of(int dim, bool direct_q, bool d
                        : grads_for<T, 128>(direct_q, direct_kv, few, few_q);
 }
 
+// Queries of a part: a step of 4096 tokens, 8 heads over 2 of 128 in bf16 under a window of 1024 takes 175 us with 512, 178 with
+// 256 and 384, 208 with 1024, 421 without parts; in 32 bits 1084, 1091, 1082 and 3618.
+constexpr int CHUNK = 512;
 // Workspace: two floats a query row and head, then the first keys' parts where they are split.
 struct GradWork { int64_t stats, part, total; int chunk; };
 static int grad_work(const spmm_attn_desc_t *a, const char *where, bool packed, GradWork *w) {
@@ -621,8 +631,11 @@ static int grad_work(const spmm_attn_desc_t *a, const char *where, bool packed, 
     w->chunk = 0;
     w->part = 0;
     const int64_t span = ((int64_t)a->window + 128 + 63) / 64 * 64;         // queries of an ordinary block of 128 keys
-    if (a->window > 0 && a->window < a->k_len && a->sinks > 0 && a->sinks <= 128 && a->k_len > a->sinks && a->q_len > 2 * span) {
-        w->chunk = (int)(span < 512 ? 512 : span);
+    // Where a sequence is longer than that, its first keys have queries beyond (2048 tokens under a window of 1024 with parts:
+    // 152 us, without: 218); a mean of the lengths, as the offsets are not known here.
+    const int64_t mean = packed && a->batch ? a->q_len / a->batch : a->q_len;
+    if (a->window > 0 && a->window < a->k_len && a->sinks > 0 && a->sinks <= 128 && a->k_len > a->sinks && mean > span) {
+        w->chunk = CHUNK;
         const int64_t slots = a->batch + (packed ? a->q_len / w->chunk + a->batch : a->batch * ((a->q_len + w->chunk - 1) / w->chunk));
         w->part = slots * a->kv_heads * 2 * a->sinks * a->dim * 4;
     }
@@ -679,7 +692,7 @@ extern "C" int spmm_attn_window_grad(const spmm_attn_desc_t *a, const spmm_attn_
     A.chunk = w.chunk;
     int qt = 0, kt = 0, ct = 0;
     const bool direct = A.k.direct && A.v.direct, direct_kv = direct && A.q.direct && A.dout.direct;
-    const bool few = (nb * a->k_len + 127) / 128 * a->kv_heads < 256, few_q = (nb * a->q_len + 127) / 128 * a->heads < 256;
+    const bool few = (nb * a->k_len + 127) / 128 * a->kv_heads < 128, few_q = (nb * a->q_len + 127) / 128 * a->heads < 256;
     const GradKernels G = a->dtype == SPMM_ATTN_F32 ? grads_of<float>(a->dim, direct, direct_kv, few, few_q)
                           : a->dtype == SPMM_ATTN_F16 ? grads_of<_Float16>(a->dim, direct, direct_kv, few, few_q)
                                                       : grads_of<__bf16>(a->dim, direct, direct_kv, few, few_q);

@@ -9,12 +9,13 @@ band plus the first columns, as two numbers.  A query at position p sees key j i
 Arguments are torch tensors on one HIP device, float32, float16 or bfloat16 alike, with the head width (1 to 128) as
 their innermost, contiguous dimension and any other strides.  Work is ordered on ``stream`` (an integer hipStream_t; by
 default the device's current stream), results and workspaces that a call allocates belong to that stream, and calls can
-be captured in a graph.  There is no CPU path.
+be captured in a graph.  What a call writes must not overlap what it reads.  There is no CPU path.
 """
 from __future__ import annotations
 
 import contextlib
 import ctypes as C
+import operator
 
 import torch
 
@@ -91,8 +92,9 @@ def _rows(t, s: tuple, packed: bool = False) -> _Rows:
 
 
 def _int(name: str, x, lo: int, hi: int = 2 ** 31 - 1) -> int:
-    if isinstance(x, bool) or not isinstance(x, int):
+    if isinstance(x, bool):
         raise TypeError(f"{name} must be an integer")
+    x = operator.index(x)
     if not lo <= x <= hi:
         raise ValueError(f"{name} = {x} is not in {lo} .. {hi}")
     return x
@@ -266,8 +268,9 @@ def paged_attention(q, k_pages, v_pages, page_table, lengths, window: int = 0, s
 def cache_append(k, v, k_pages, v_pages, page_table, lengths, cu=None, stream: int | None = None) -> None:
     """Write the keys and values of new tokens into the cache: those of sequence b go to its last positions before
     ``lengths[b]``.  k and v [batch, key heads, d], one token a sequence (none for a sequence of length 0), or, with
-    int32 offsets ``cu`` [batch + 1] on the device, [rows, key heads, d].  Rows whose page is not there are dropped.  A
-    page that is written must belong to one sequence only."""
+    int32 offsets ``cu`` [batch + 1] on the device, [rows, key heads, d].  Rows whose page is not there are dropped, and
+    all rows of a sequence whose length is above what the table can hold.  A page that is written must belong to one
+    sequence only."""
     ks = _tensor("k", k)
     dev, dt = k.get_device(), k.dtype
     vs = _tensor("v", v, dt, dev, k.shape)

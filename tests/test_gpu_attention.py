@@ -492,3 +492,57 @@ def test_masked_places_do_not_leak_in_large_blocks(A, dtype, value):
             other = torch.arange(n) != where
             assert all(torch.equal(got[j][0][other], ref[j][0][other]) for j in (0, 2))
             assert all(torch.equal(got[j][0][keys], ref[j][0][keys]) for j in (3, 4))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_hidden_values_of_several_tiles(A, dtype):
+    """Values that are not finite in tile after tile, some at the start and some at the end of what a block takes: every
+    wave of a block has to take the careful way at the same place, each time."""
+    n, h, hk, d, window, sinks = 420, 4, 2, 64, 48, 3
+    base = [rnd(i, 1, n, h if i in (1, 4) else hk, d, dtype=dtype) for i in (1, 2, 3, 4)]
+    at = torch.tensor([20, 64, 95, 127, 128, 161, 192, 255, 256, 300, 319])
+    run = lambda q, k, v, do: (lambda o, l: (o, l) + A.window_attention_backward(do, q, k, v, o, l, window, sinks))(
+        *A.window_attention(q, k, v, window, sinks))
+    ref = run(*base)
+    seen = O.visible(n, n, window, sinks)
+    rows = ~seen[:, at].any(1)
+    x = [t.clone() for t in base]
+    x[1][:, at, :, 3] = x[2][:, at, :, 60] = math.nan
+    first = run(*x)
+    assert int(rows.sum()) > 60
+    assert all(torch.equal(first[j][0][rows], ref[j][0][rows]) for j in (0, 1, 2))
+    assert all(not torch.isfinite(first[j][0][~rows]).all(-1).any() for j in (0, 2))
+    for _ in range(5):
+        assert all(torch.equal(a.nan_to_num(7.0), b.nan_to_num(7.0)) for a, b in zip(run(*x), first))
+
+
+@pytest.mark.parametrize("cuts", [(0, 900), (0, 1, 2, 900), (0, 880, 890, 900)], ids=str)
+def test_first_keys_of_long_and_short_sequences(A, cuts):
+    """The first keys' gradients where the mean length is on either side of what has their queries split."""
+    n, h, hk, d, window, sinks = cuts[-1], 4, 2, 64, 40, 4
+    q, k, v, do = (rnd(i, n, h if i in (1, 4) else hk, d, dtype=F16) for i in (1, 2, 3, 4))
+    cu = torch.tensor(cuts, dtype=torch.int32).cuda()
+    out, lse = A.window_attention(q, k, v, window, sinks, cu_q=cu)
+    got = A.window_attention_backward(do, q, k, v, out, lse, window, sinks, cu_q=cu)
+    for a, b in zip(cuts, cuts[1:]):
+        s = slice(a, b)
+        r = O.attention(q[s], k[s], v[s], window, sinks)
+        O.check("out", out[s], r["out"], r["tol_out"])
+        g = O.gradients(r, do[s])
+        for name, x in zip(("dq", "dk", "dv"), got):
+            O.check(name, x[s], g[name], g["tol_" + name])
+
+
+def test_append_to_a_table_of_one_column(A):
+    kp, vp = (torch.zeros(3, 4, 2, 8, device="cuda") for _ in range(2))
+    k = rnd(1, 3, 2, 8)
+    table = torch.tensor([[2], [0], [1]], dtype=torch.int32).cuda()
+    A.cache_append(k, k, kp, vp, table, torch.tensor([4, 5, 0], dtype=torch.int32).cuda())      # the last, one too far, none
+    assert torch.equal(kp[2, 3], k[0]) and torch.equal(vp[2, 3], k[0]) and int((kp != 0).sum()) == 16 == int((vp != 0).sum())
+
+
+def test_integers_of_other_libraries(A):
+    import numpy as np
+    q = rnd(1, 1, 40, 2, 16)
+    a, b = A.window_attention(q, q, q, 8, 2), A.window_attention(q, q, q, np.int64(8), np.int32(2))
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
