@@ -17,7 +17,8 @@
  * SPMM_ATTN_BF16; scores, softmax statistics and sums are 32-bit floats.  With the 16-bit types spmm_attn_window rounds
  * the weights to that type before they enter a product, and spmm_attn_window_grad the weights and their gradients where
  * they enter dv and dk; in dq and in spmm_attn_paged they enter as a rounded value plus its rounded remainder.  Results
- * do not depend on anything but the arguments: no atomics, fixed orders of summation.
+ * do not depend on anything but the arguments: no atomics, fixed orders of summation (in spmm_attn_paged the order is
+ * a matter of all the lengths).
  *
  * Every pointer is a device address on `device`, and what a call writes does not overlap what it reads.  Calls are
  * ordered on `stream` (a hipStream_t, NULL = the null stream), hold no state between calls and can be captured in a

@@ -9,19 +9,20 @@
 //    operand of a 16x16x16 product (of four 16x16x4 ones in 32 bits), whose second operand is element j of value rows
 //    4 (l / 16) + 0..3: lane l % 16 loads a piece of those four rows, and element j of each makes up product j.  The
 //    values need no transposition.  16-bit products take the weights in two parts, so they lose nothing by rounding.
-// A block's four waves share a stretch of the keys and join through LDS; when there are few sequences the keys are
-// split over several blocks, and a second kernel joins their parts in order.
+// A block's four waves share a stretch of the keys and join through LDS.  Where sequences are longer than a block should
+// take alone, all of them are cut into parts of about one length by what the lengths say, as many as the compute units
+// hold at once, and a second kernel joins the parts of a sequence in order.
 #include "attn_common.hpp"
 
 namespace attn {
 
 constexpr int PW = 4;                        // waves of a block
 constexpr int PK = 16;                       // keys a wave takes at a time
-constexpr int ALONE = 256;                   // keys up to which a block takes a sequence alone
+constexpr int ALONE = 256;                   // keys up to which nothing is cut: a second launch costs more
 constexpr int SPLIT_MIN = 64;                // keys a block takes at least otherwise: one tile a wave
 constexpr int SPLIT_MAX = 256;               // parts of a sequence at most
 // blocks that a compute unit holds at once
-__host__ __device__ constexpr int paged_blocks(bool half) { return half ? 4 : 2; }
+__host__ __device__ constexpr int paged_blocks(bool half) { return half ? 4 : 3; }
 
 struct PagedArgs {
     Rows q, out;
@@ -30,9 +31,11 @@ struct PagedArgs {
     const int32_t *table, *lengths;
     bool k_wide, v_wide;
     int64_t batch, limit;                    // limit: longest sequence allowed
-    int heads, kv_heads, dim, window, sinks, splits, page_shift;      // page_shift: of a power of two, else -1
+    int heads, kv_heads, dim, window, sinks, page_shift;      // page_shift: of a power of two, else -1
+    int room, cap;                           // parts wanted of all sequences (0: they are not cut), and room for them
     float scale2;
-    float *lse, *part;                       // part: [batch][heads][splits][dim + 2]: max, sum, weighted values
+    int32_t *start;                          // [batch][2] of a sequence: its first part, and how many
+    float *lse, *part;                       // part: [heads][cap][2] max, sum, then [heads][cap][dim] weighted values
 };
 
 // The 16-key tiles that hold visible keys: `first` tiles from position 0, then those from `start` on.
@@ -47,6 +50,46 @@ __device__ __forceinline__ Span span_of(int len, int window, int sinks) {
     s.first = min((min(sinks, len) + PK - 1) / PK, s.start);
     s.tiles = s.first + (len + PK - 1) / PK - s.start;
     return s;
+}
+
+// The cut of the sequences into parts: each into equal ones of `per` tiles at most, SPLIT_MAX of them at most.  Every wave
+// works it out from the lengths.  With per = total / room + 1 there are room + batch parts at most.  With up to 64 sequences
+// it is the smallest, but for 3 %, that makes them `room`, if 2 per does: a few blocks more than the compute units hold at
+// once would take as long again, and a longer part is what the others wait for.  Next to as many parts for every
+// sequence this costs about 2 us and gains where lengths differ: 17 sequences of 1 to 23493 keys, 32 heads over 4 of 96 in 32
+// bits, 206 -> 68 us, 9 of 7 to 19511, 8 heads over 8 of 96 in fp16, 64 -> 46; 1000 keys of one sequence 9.8 -> 11.3.
+__device__ __forceinline__ int tiles_of(const PagedArgs &A, int64_t b) {
+    const int len = b < A.batch ? A.lengths[b] : 0;
+    return len < 0 || len > A.limit ? 0 : span_of(len, A.window, A.sinks).tiles;
+}
+__device__ __forceinline__ int parts_of(int tiles, int per) {
+    return min(max(1, (int)(((uint32_t)tiles + per - 1) / (uint32_t)per)), SPLIT_MAX);
+}
+// first: tiles of sequence `lane`
+__device__ __forceinline__ int plan(const PagedArgs &A, int lane, int first) {
+    if (A.batch <= WAVE) {                                  // the tiles of 64 sequences are less than 2^32
+        uint32_t total = first;
+#pragma unroll
+        for (int d = 32; d; d /= 2) total += __shfl_xor(total, d);
+        const int lo = max(SPLIT_MIN / PK, (int)((uint32_t)uniform((int)total) / (uint32_t)A.room) + 1);
+        auto fits = [&](int per) {
+            const int n = lane < A.batch ? parts_of(first, per) : 0;      // 256 at most
+            int sum = 0;
+#pragma unroll
+            for (int bit = 0; bit <= 8; ++bit) sum += __popcll(__ballot(n >> bit & 1)) << bit;
+            return sum <= A.room;
+        };
+        if (fits(lo) || !fits(2 * lo)) return lo;
+        int per = 2 * lo;
+        for (int step = lo / 2, i = 0; i < 5 && step > 0; step /= 2, ++i)
+            if (fits(per - step)) per -= step;
+        return per;
+    }
+    int64_t total = first;
+    for (int64_t b = lane + WAVE; b < A.batch; b += WAVE) total += tiles_of(A, b);
+#pragma unroll
+    for (int d = 32; d; d /= 2) total += __shfl_xor(total, d);
+    return uniform(max(SPLIT_MIN / PK, (int)min(total / A.room, (int64_t)INT32_MAX - 1) + 1));
 }
 
 // Depth 16: lane l gives row (column) l % 16 at depths 4 (l / 16) + 0..3.
@@ -98,6 +141,24 @@ __device__ __forceinline__ void add_values(f32x4 (&o)[VE], const f32x4 &w, const
     }
 }
 
+// Values that are not finite, taken out of the pieces and added by themselves: with a weight that was rounded to 0, or as its
+// remainder is, the products would make NaN of an infinity.
+template <typename T, int VE> __device__ __forceinline__ void add_not_finite(f32x4 (&o)[VE], typename Piece<T, VE>::vec (&v)[4]) {
+#pragma unroll
+    for (int j = 0; j < VE; ++j) {
+        float x = 0.f;
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            if (!finite_f((float)v[r][j])) {
+                x += (float)v[r][j];
+                v[r][j] = (T)0.f;
+            }
+        x += __shfl_xor(x, 16);
+        x += __shfl_xor(x, 32);
+        o[j] += x;
+    }
+}
+
 template <typename T, int DP>
 __global__ __launch_bounds__(PW * 64, paged_blocks(sizeof(T) == 2)) void paged_kernel(PagedArgs A) {
     // a lane's columns of the values: VE from VE (lane % 16) on
@@ -107,14 +168,42 @@ __global__ __launch_bounds__(PW * 64, paged_blocks(sizeof(T) == 2)) void paged_k
     int id = (int)blockIdx.x;
     const int kv = id % A.kv_heads; id /= A.kv_heads;
     const int g0 = id % hb * 16; id /= hb;
-    const int split = id % A.splits;
-    const int64_t b = id / A.splits;
+    int64_t b = id;
+    int per = 0, split = 0, parts = 1;                      // tiles of a part, which one this is, of how many
+    if (A.room) {
+        const int first = tiles_of(A, lane), part_tile = plan(A, lane, first);
+        int before = 0;
+        for (b = 0;; b += WAVE) {
+            if (b >= A.batch) return;                       // fewer parts than there could be
+            const int tiles = b ? tiles_of(A, b + lane) : first, n0 = b + lane < A.batch ? parts_of(tiles, part_tile) : 0;
+            int incl = n0;
+#pragma unroll
+            for (int d = 1; d < WAVE; d *= 2) {
+                const int o = __shfl_up(incl, d);
+                if (lane >= d) incl += o;
+            }
+            const unsigned long long hit = __ballot(before + incl > id);
+            if (hit) {
+                const int src = __ffsll(hit) - 1;
+                b += src;
+                split = uniform(id - before - __shfl(incl - n0, src));
+                parts = uniform(__shfl(n0, src));
+                per = (uniform(__shfl(tiles, src)) + parts - 1) / parts;
+                if (split == 0 && kv == 0 && g0 == 0 && threadIdx.x == 0) {
+                    A.start[2 * b] = id;
+                    A.start[2 * b + 1] = parts;
+                }
+                break;
+            }
+            before += uniform(__shfl(incl, WAVE - 1));
+        }
+    }
 
     int len = A.lengths[b];
     bool bad = len < 0 || len > A.limit;
     if (bad) len = 0;
     const Span sp = span_of(len, A.window, A.sinks);
-    const int per = (sp.tiles + A.splits - 1) / A.splits, t0 = split * per, t1 = min(t0 + per, sp.tiles);
+    const int t0 = split * per, t1 = A.room ? min(t0 + per, sp.tiles) : sp.tiles;
 
     const int head = kv * group + g0 + n;
     const bool mine = g0 + n < group;
@@ -144,53 +233,65 @@ __global__ __launch_bounds__(PW * 64, paged_blocks(sizeof(T) == 2)) void paged_k
     };
 
     f32x4 o[VE];
+    float m, sum;
+    // A second time, and with care, if some sum is NaN in the end: each wave for itself.
+    for (bool careful = false;; careful = true) {
 #pragma unroll
-    for (int j = 0; j < VE; ++j) o[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    float m = -INFINITY, sum = 0.f;
-    int slot_next, page_next = locate(t0 + wave, slot_next);
-    for (int t = t0 + wave; t < t1; t += PW) {
-        const int j0 = sp.at(t), page = page_next, slot = slot_next;
-        page_next = locate(t + PW, slot_next);
-        bad |= page == -2;
-        const int64_t voff = page < 0 ? -1 : (int64_t)page * A.v_page + slot * A.v_row;
-        const T *kr = page < 0 ? (const T *)zero_row : kb + (int64_t)page * A.k_page + slot * A.k_row;
-        frag<T> kf[NS];
+        for (int j = 0; j < VE; ++j) o[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+        m = -INFINITY;
+        sum = 0.f;
+        int slot_next, page_next = locate(t0 + wave, slot_next);
+        for (int t = t0 + wave; t < t1; t += PW) {
+            const int j0 = sp.at(t), page = page_next, slot = slot_next;
+            page_next = locate(t + PW, slot_next);
+            bad |= page == -2;
+            const int64_t voff = page < 0 ? -1 : (int64_t)page * A.v_page + slot * A.v_row;
+            const T *kr = page < 0 ? (const T *)zero_row : kb + (int64_t)page * A.k_page + slot * A.k_row;
+            frag<T> kf[NS];
 #pragma unroll
-        for (int s = 0; s < NS; ++s) kf[s] = Piece<T, 8>::load(kr, s * 32 + h4 * 8, A.dim, A.k_wide);
-        typename Piece<T, VE>::vec vr[4];
+            for (int s = 0; s < NS; ++s) kf[s] = Piece<T, 8>::load(kr, s * 32 + h4 * 8, A.dim, A.k_wide);
+            typename Piece<T, VE>::vec vr[4];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int64_t off = __shfl(voff, 4 * h4 + r);
-            vr[r] = Piece<T, VE>::load(off < 0 ? (const T *)zero_row : vb + off, n * VE, A.dim, A.v_wide);
+            for (int r = 0; r < 4; ++r) {
+                const int64_t off = __shfl(voff, 4 * h4 + r);
+                vr[r] = Piece<T, VE>::load(off < 0 ? (const T *)zero_row : vb + off, n * VE, A.dim, A.v_wide);
+            }
+            f32x4 sc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int s = 0; s < NS; ++s) sc = mma16(kf[s], qf[s], sc);
+            float mx = m;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                sc[r] = seen(j0 + 4 * h4 + r) ? sc[r] * A.scale2 : -INFINITY;
+                mx = fmaxf(mx, sc[r]);
+            }
+            mx = fmaxf(mx, __shfl_xor(mx, 16));
+            mx = fmaxf(mx, __shfl_xor(mx, 32));
+            const float base = mx == -INFINITY ? 0.f : mx;
+            if (__any(mx != m)) {
+                const float alpha = __builtin_amdgcn_exp2f(m - base);
+                sum *= alpha;
+                f32x4 a4;                                       // accumulator rows are heads 4 h4 + r
+#pragma unroll
+                for (int r = 0; r < 4; ++r) a4[r] = __shfl(alpha, 4 * h4 + r);
+#pragma unroll
+                for (int j = 0; j < VE; ++j) o[j] *= a4;
+                m = mx;
+            }
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                sc[r] = __builtin_amdgcn_exp2f(sc[r] - base);
+                sum += sc[r];
+            }
+            if (careful) add_not_finite<T, VE>(o, vr);
+            add_values<T, VE>(o, sc, vr);
         }
-        f32x4 sc = {0.f, 0.f, 0.f, 0.f};
+        bool nan = false;
 #pragma unroll
-        for (int s = 0; s < NS; ++s) sc = mma16(kf[s], qf[s], sc);
-        float mx = m;
+        for (int j = 0; j < VE; ++j)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            sc[r] = seen(j0 + 4 * h4 + r) ? sc[r] * A.scale2 : -INFINITY;
-            mx = fmaxf(mx, sc[r]);
-        }
-        mx = fmaxf(mx, __shfl_xor(mx, 16));
-        mx = fmaxf(mx, __shfl_xor(mx, 32));
-        const float base = mx == -INFINITY ? 0.f : mx;
-        if (__any(mx != m)) {
-            const float alpha = __builtin_amdgcn_exp2f(m - base);
-            sum *= alpha;
-            f32x4 a4;                                       // accumulator rows are heads 4 h4 + r
-#pragma unroll
-            for (int r = 0; r < 4; ++r) a4[r] = __shfl(alpha, 4 * h4 + r);
-#pragma unroll
-            for (int j = 0; j < VE; ++j) o[j] *= a4;
-            m = mx;
-        }
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            sc[r] = __builtin_amdgcn_exp2f(sc[r] - base);
-            sum += sc[r];
-        }
-        add_values<T, VE>(o, sc, vr);
+            for (int r = 0; r < 4; ++r) nan |= o[j][r] != o[j][r];
+        if (careful || !__any(nan)) break;
     }
     sum += __shfl_xor(sum, 16);
     sum += __shfl_xor(sum, 32);
@@ -223,16 +324,16 @@ __global__ __launch_bounds__(PW * 64, paged_blocks(sizeof(T) == 2)) void paged_k
             acc += f * so[w][hh][d];
         }
         const int hd = kv * group + g0 + hh;
-        if (A.splits == 1) {
+        if (parts == 1) {
             ((T *)A.out.ptr)[b * A.out.seq + hd * A.out.head + d] = narrow<T>(tot == 0.f ? 0.f : acc / tot);
             if (d == 0) A.lse[b * A.heads + hd] = tot == 0.f ? -INFINITY : mx * LN2 + __logf(tot);
         } else {
-            float *p = A.part + ((b * A.heads + hd) * A.splits + split) * (A.dim + 2);
+            const int64_t at = (int64_t)hd * A.cap + id;
             if (d == 0) {
-                p[0] = mx;
-                p[1] = tot;
+                A.part[2 * at] = mx;
+                A.part[2 * at + 1] = tot;
             }
-            p[2 + d] = acc;
+            A.part[2 * (int64_t)A.heads * A.cap + at * A.dim + d] = acc;
         }
     }
 }
@@ -242,48 +343,59 @@ __global__ __launch_bounds__(PW * 64, paged_blocks(sizeof(T) == 2)) void paged_k
 constexpr int JW = 4;
 template <typename T> __global__ __launch_bounds__(JW * 64) void paged_join_kernel(PagedArgs A) {
     const int64_t x = blockIdx.x, b = x / A.heads;
-    const int hd = (int)(x % A.heads), lane = threadIdx.x & 63, wave = threadIdx.x >> 6, w = A.dim + 2;
-    const float *p = A.part + x * A.splits * w;
+    const int hd = (int)(x % A.heads), lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int splits = A.start[2 * b + 1];
+    if (splits == 1) return;                                // the block that took it has stored the result
+    const int64_t at = (int64_t)hd * A.cap + A.start[2 * b];
+    const float *st = A.part + 2 * at, *p = A.part + 2 * (int64_t)A.heads * A.cap + at * A.dim;
     float mx = -INFINITY;
-    for (int s = lane; s < A.splits; s += WAVE) mx = fmaxf(mx, p[(int64_t)s * w]);
+    for (int s = lane; s < splits; s += WAVE) mx = fmaxf(mx, st[2 * s]);
 #pragma unroll
     for (int d = 32; d; d /= 2) mx = fmaxf(mx, __shfl_xor(mx, d));
     const float base = mx == -INFINITY ? 0.f : mx;
     float tot = 0.f, a0 = 0.f, a1 = 0.f;
     const int e0 = min(lane, A.dim - 1), e1 = min(lane + WAVE, A.dim - 1);
-    const int per = (A.splits + JW - 1) / JW, last = min((wave + 1) * per, A.splits);
+    const int per = (splits + JW - 1) / JW, last = min((wave + 1) * per, splits);
     for (int s0 = wave * per; s0 < last; s0 += WAVE) {
         const int n = min(WAVE, last - s0);
-        const float *ps = p + (int64_t)s0 * w;
+        const float *ps = p + (int64_t)s0 * A.dim;
         float f = 0.f, add = 0.f;
         if (lane < n) {
-            f = __builtin_amdgcn_exp2f(ps[lane * w] - base);
-            add = f * ps[lane * w + 1];
+            f = __builtin_amdgcn_exp2f(st[2 * (s0 + lane)] - base);
+            add = f * st[2 * (s0 + lane) + 1];
         }
 #pragma unroll
         for (int d = 32; d; d /= 2) add += __shfl_xor(add, d);
         tot += add;
         for (int s = 0; s < n; s += 8) {
+            float y0[8], y1[8];                             // all asked for before any is used; past the last part that one again
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {                   // past the last part: its values times 0
+            for (int i = 0; i < 8; ++i) {
+                const float *pi = ps + min(s + i, n - 1) * A.dim;
+                y0[i] = pi[e0];
+                y1[i] = pi[e1];
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) asm volatile("" : "+v"(y0[i]), "+v"(y1[i]));
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
                 const float fs = __shfl(f, s + i);
-                const float *pi = ps + min(s + i, n - 1) * w + 2;
-                a0 += fs * pi[e0];
-                a1 += fs * pi[e1];
+                a0 = s + i < n ? a0 + fs * y0[i] : a0;
+                a1 = s + i < n ? a1 + fs * y1[i] : a1;
             }
         }
     }
-    __shared__ float st[JW], s0[JW][WAVE], s1[JW][WAVE];
-    if (lane == 0) st[wave] = tot;
-    s0[wave][lane] = a0;
-    s1[wave][lane] = a1;
+    __shared__ float wt[JW], w0[JW][WAVE], w1[JW][WAVE];
+    if (lane == 0) wt[wave] = tot;
+    w0[wave][lane] = a0;
+    w1[wave][lane] = a1;
     __syncthreads();
     if (wave) return;
 #pragma unroll
     for (int i = 1; i < JW; ++i) {
-        tot += st[i];
-        a0 += s0[i][lane];
-        a1 += s1[i][lane];
+        tot += wt[i];
+        a0 += w0[i][lane];
+        a1 += w1[i][lane];
     }
     const float inv = tot == 0.f ? 0.f : 1.f / tot;
     T *dst = (T *)A.out.ptr + b * A.out.seq + hd * A.out.head;
@@ -370,19 +482,23 @@ static int check_pages(const spmm_attn_desc_t *a, const spmm_attn_pages_t *p, co
     return SPMM_HIP_OK;
 }
 
-// Blocks that share a sequence's keys: as many as are on the compute units at once (four each, two with 32-bit elements), each
-// with SPLIT_MIN keys or more, SPLIT_MAX parts at most; none share up to ALONE keys, where a second launch costs more.
-// In bf16, 8 heads over 1 of 128: 1000 keys 9.8 us (parts of 128 keys 11.2, of 256 14.2, of 512 20.2), 8192 keys 11.7 (20.5 with
-// 512); 2 key heads, 100000 keys 30.5 us with 256 parts (35 with 128 or 512).  Batch of 32 of 4096 keys, 32 heads over 8:
-// 1024 blocks 108 us, 512 blocks 115, 2048 blocks 111; in 32 bits 512 blocks 250, 256 blocks 390.
-static int64_t split_count(const spmm_attn_desc_t *a, int64_t max_length) {
-    const int64_t group = a->heads / a->kv_heads, base = a->batch * a->kv_heads * ((group + 15) / 16);
+// Parts wanted of all sequences (0: they are not cut) and the most there can be: as many blocks as are on the compute units at
+// once (four each, three with 32-bit elements), each part of SPLIT_MIN keys or more, SPLIT_MAX a sequence at most.
+// In bf16, 8 heads over 1 of 128: 1000 keys 11.3 us with parts of 64 keys, 1.4 more with 128, 4.4 with 256, 10 with 512; 2 key
+// heads, 100000 keys 33 us with 256 parts, 4.5 more with 128 or 512.  Batch of 32 of 4096 keys, 32 heads over 8: 1024 blocks
+// 111 us, 512 blocks 4 % more, 2048 blocks 3 %; in 32 bits 768 blocks 210, 512 blocks 250, 1024 280.
+static void cut(const spmm_attn_desc_t *a, int64_t max_length, int *room, int64_t *parts) {
+    const int64_t group = a->heads / a->kv_heads, each = a->kv_heads * ((group + 15) / 16);
     int64_t keys = max_length;
     if (a->window && a->window < keys) keys = (int64_t)a->window + (a->sinks < keys - a->window ? a->sinks : keys - a->window);
-    const int64_t most = (keys + SPLIT_MIN - 1) / SPLIT_MIN, want = base > 0 ? 256 * paged_blocks(a->dtype != SPMM_ATTN_F32) / base : 1;
-    int64_t n = want < most ? want : most;
-    n = n < SPLIT_MAX ? n : SPLIT_MAX;
-    return n < 1 || keys <= ALONE ? 1 : n;
+    *room = 0;
+    *parts = a->batch;
+    if (keys <= ALONE) return;
+    const int64_t want = 256 * paged_blocks(a->dtype != SPMM_ATTN_F32) / each;
+    *room = want > 1 ? (int)want : 1;
+    // first keys and window: up to three tiles more than their number asks for
+    const int64_t most = (keys + 3 * PK + SPLIT_MIN - 1) / SPLIT_MIN, n = a->batch * (most < SPLIT_MAX ? most : SPLIT_MAX);
+    *parts = n < *room + a->batch ? n : *room + a->batch;
 }
 
 template <typename T> static const void *paged_of(int dim) {
@@ -398,8 +514,10 @@ extern "C" int spmm_attn_paged_work(const spmm_attn_desc_t *a, int64_t max_lengt
     if (st != SPMM_HIP_OK) return st;
     if (!bytes || max_length < 0 || max_length > INT32_MAX / 2)
         return fail(SPMM_HIP_ERR_ARG, "attn_paged_work: bytes is NULL, or max_length %lld", (long long)max_length);
-    const int64_t s = split_count(a, max_length);
-    *bytes = s > 1 ? (size_t)(a->batch * a->heads * s * (a->dim + 2)) * 4 : 0;
+    int room;
+    int64_t parts;
+    cut(a, max_length, &room, &parts);
+    *bytes = room ? (size_t)((a->batch + 1) / 2 * 4 + parts * a->heads * (a->dim + 2)) * 4 : 0;
     return SPMM_HIP_OK;
 }
 
@@ -444,11 +562,15 @@ extern "C" int spmm_attn_paged(const spmm_attn_desc_t *a, const spmm_attn_rows_t
     A.dim = a->dim;
     A.window = a->window;
     A.sinks = a->window ? a->sinks : 0;
-    A.splits = (int)split_count(a, max_length);
+    int64_t parts;
+    cut(a, max_length, &A.room, &parts);
+    if (parts > INT32_MAX) return fail(SPMM_HIP_ERR_OVERFLOW, "%s: too many parts", W);
+    A.cap = (int)parts;
     A.page_shift = A.page_rows & (A.page_rows - 1) ? -1 : __builtin_ctzll((unsigned long long)A.page_rows);
     A.scale2 = a->scale * LOG2E;
     A.lse = lse;
-    A.part = (float *)work;
+    A.start = (int32_t *)work;
+    A.part = (float *)work + (a->batch + 1) / 2 * 4;
     OnDevice on(a->device, W);
     if (on.status) return on.status;
     const void *kern = a->dtype == SPMM_ATTN_F32 ? paged_of<float>(a->dim)
@@ -458,8 +580,8 @@ extern "C" int spmm_attn_paged(const spmm_attn_desc_t *a, const spmm_attn_rows_t
                                                    : (const void *)paged_join_kernel<__bf16>;
     void *args[] = {&A};
     const int64_t hb = (a->heads / a->kv_heads + 15) / 16;
-    if ((st = launch(kern, W, a->batch * A.splits * hb * a->kv_heads, PW * 64, args, stream))) return st;
-    return A.splits > 1 ? launch(join, W, a->batch * a->heads, JW * 64, args, stream) : SPMM_HIP_OK;
+    if ((st = launch(kern, W, parts * hb * a->kv_heads, PW * 64, args, stream))) return st;
+    return A.room ? launch(join, W, a->batch * a->heads, JW * 64, args, stream) : SPMM_HIP_OK;
 }
 
 extern "C" int spmm_attn_append(const spmm_attn_desc_t *a, const spmm_attn_rows_t *k, const spmm_attn_rows_t *v,

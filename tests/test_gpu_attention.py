@@ -546,3 +546,43 @@ def test_integers_of_other_libraries(A):
     q = rnd(1, 1, 40, 2, 16)
     a, b = A.window_attention(q, q, q, 8, 2), A.window_attention(q, q, q, np.int64(8), np.int32(2))
     assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+# long and short sequences together: more than 64, more parts than one sequence may have, more sequences than parts are wanted
+CUT = [
+    ([9000] + [1 + 7 * i for i in range(69)], 4, 2, 64, 16, 0, 0), ([20000], 2, 1, 32, 64, 0, 0),
+    ([300 - 3 * i for i in range(40)], 64, 64, 8, 16, 0, 0), ([6001, 0, 1, 2500, 63, 64, 65, 900], 24, 1, 128, 32, 0, 0),
+    ([6001, 3, 4000, 1500] * 5, 8, 8, 80, 16, 1000, 40),
+]
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("case", CUT, ids=lambda c: str(c)[:40])
+def test_paged_mixed_lengths(A, case, dtype):
+    lens, h, hk, d, page, window, sinks = case
+    kp, vp, table, lengths, ks, vs = make_cache(lens, page, hk, d, dtype)
+    q = rnd(5, len(lens), h, d, dtype=dtype)
+    out, lse = A.paged_attention(q, kp, vp, table, lengths, window, sinks)
+    check_paged(A, q, ks, vs, out, lse, window, sinks)
+    again, lse2 = A.paged_attention(q, kp, vp, table, lengths, window, sinks)
+    assert torch.equal(out, again) and torch.equal(lse, lse2)
+
+
+def test_paged_bad_length_among_long_ones(A):
+    lens = [4000, 700, 2000]
+    kp, vp, table, lengths, ks, vs = make_cache(lens, 16, 2, 64, BF16)
+    q = rnd(5, 3, 4, 64, dtype=BF16)
+    lengths[1] = -4
+    out, lse = A.paged_attention(q, kp, vp, table, lengths)
+    assert out[1].isnan().all() and lse[1].isnan().all()
+    check_paged(A, q[::2], ks[::2], vs[::2], out[::2], lse[::2], 0, 0)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_paged_infinite_value_in_the_last_part(A, dtype):
+    lens = [1100]
+    kp, vp, table, lengths, ks, vs = make_cache(lens, 16, 1, 64, dtype)
+    q = rnd(5, 1, 2, 64, dtype=dtype)
+    vp[table[0, 1099 // 16], 1099 % 16, 0, 5] = math.inf
+    out, lse = A.paged_attention(q, kp, vp, table, lengths)
+    assert (out[0, :, 5] == math.inf).all() and torch.isfinite(out[0, :, :5]).all() and torch.isfinite(lse).all()
