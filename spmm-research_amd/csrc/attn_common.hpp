@@ -253,10 +253,6 @@ struct Mask {
     __device__ __forceinline__ bool all(int p0, int p1, int j0, int j1) const {
         return j1 <= p0 && (window == 0 || p1 - j0 < window || j1 < sinks);
     }
-    // some (p, j) of [p0, p1] x [j0, j1] visible (j0 <= j1)
-    __device__ __forceinline__ bool any(int p0, int p1, int j0, int j1) const {
-        return j0 <= p1 && (window == 0 || j0 < sinks || p0 - j1 < window);
-    }
 };
 
 // ------------------------------------------------------------------------------------------------ sequences

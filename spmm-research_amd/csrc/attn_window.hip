@@ -5,6 +5,15 @@
 // lane owns one query (column l % 32) and half of the tile's keys: the softmax statistics of a query need one exchange
 // between two lanes, and S^T leaves the matrix unit in the layout in which exp(S^T) is the second operand of
 // O^T = V^T P^T -- the weights never pass through LDS.  V^T comes from the row-major tile by the transposing LDS read.
+//
+// The weights of 16-bit types are rounded to the type for the second product, at most 2^-8 (bf16) or 2^-11 (fp16) of each,
+// as the values are; their sum is taken before that, in 32 bits.
+//
+// Bound: matrix instructions and the exponentials beside them, which do not overlap within a wave; two blocks a compute
+// unit fill the gaps of each other.  One sequence of 16384 tokens, 32 heads over 8 of 128 in bf16, window 2048, 16 first
+// keys: 610 us, 850 TFLOP/s of products (a plain product of 8192^3 reaches 1127).  128 queries a block: with 256 (eight waves)
+// 699 to 728 us.  Loading the next tile's fragments ahead, unrolling by two tiles and raised wave priority gained
+// nothing.  A ragged batch of eight of 0 to 2051 tokens, 16 heads over 4 of 80: 38 us, with 64 queries a block 41 to 48.
 #include "attn_window.hpp"
 
 namespace attn {

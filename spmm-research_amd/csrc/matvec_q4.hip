@@ -9,6 +9,8 @@
 // 16 is the smallest such offset, so little is lost in that difference (2^-24 * 31 / |q - zero| relative to a group's
 // sum of |w x|).  32-bit x is split into three bfloat16 parts of 8 bits each that sum to it exactly and take three of
 // the 16 columns.
+// Four vectors in fp16 with 16384 x 8192 weights in groups of 128 with zero points: 17.7 us, 4.0 TB/s; one in 32 bits with
+// 512 x 512 in groups of 32: 6.6 us, nearly all of it the launch and two memory latencies.
 #include <hip/hip_runtime.h>
 
 #include <cstdarg>
