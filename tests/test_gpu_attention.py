@@ -586,3 +586,40 @@ def test_paged_infinite_value_in_the_last_part(A, dtype):
     vp[table[0, 1099 // 16], 1099 % 16, 0, 5] = math.inf
     out, lse = A.paged_attention(q, kp, vp, table, lengths)
     assert (out[0, :, 5] == math.inf).all() and torch.isfinite(out[0, :, :5]).all() and torch.isfinite(lse).all()
+
+
+def test_paged_graph_follows_the_lengths(A):
+    """A captured call replayed as the sequences grow and shrink: the cut into parts is taken anew each time."""
+    full = [5000, 300, 4000, 2500]
+    kp, vp, table, lengths, ks, vs = make_cache(full, 32, 2, 64, BF16)
+    q = rnd(5, 4, 8, 64, dtype=BF16)
+    lengths[:] = 1
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        A.paged_attention(q, kp, vp, table, lengths)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out, lse = A.paged_attention(q, kp, vp, table, lengths)
+    for now in ([1, 1, 1, 1], full, [0, 300, 17, 2500], [4999, 1, 0, 0], full):
+        lengths.copy_(torch.tensor(now, dtype=torch.int32))
+        g.replay()
+        torch.cuda.synchronize()
+        check_paged(A, q, [k[:n] for k, n in zip(ks, now)], [v[:n] for v, n in zip(vs, now)], out, lse, 0, 0)
+        eager, l2 = A.paged_attention(q, kp, vp, table, lengths)
+        assert torch.equal(out, eager) and torch.equal(lse, l2)
+
+
+def test_paged_on_two_streams(A):
+    lens = [3000, 40, 900]
+    kp, vp, table, lengths, ks, vs = make_cache(lens, 16, 2, 64, F16)
+    qs = [rnd(i, 3, 4, 64, dtype=F16) for i in range(4)]
+    want = [A.paged_attention(q, kp, vp, table, lengths) for q in qs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(3):
+        got = [A.paged_attention(q, kp, vp, table, lengths, stream=streams[i % 2].cuda_stream) for i, q in enumerate(qs)]
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for x, y in zip(got, want) for a, b in zip(x, y))
