@@ -11,7 +11,7 @@
 //
 // Bound: matrix instructions, exponentials and the reads of LDS that feed them.  Two sequences of 8192 and 8000 tokens, 32
 // heads over 8 of 128 in bf16, window 1024, 4 first keys: delta 51 us (the bytes of out and dout), grad_q 602, grad_kv 795,
-// join 15; with the forward pass 1750 us, 510 TFLOP/s of the five products that the formulas need.  Keeping V's
+// join 15; with the forward pass 1750 us, 510 TFLOP/s of the seven products that the formulas need.  Keeping V's
 // fragments in registers as well, or two half tiles in turn, spills and is slower (2455 and 2300 us).
 #include "attn_window.hpp"
 

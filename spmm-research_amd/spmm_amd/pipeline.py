@@ -195,7 +195,7 @@ class TokenPipeline:
 
     def prompt(self, x, cu, page_table, lengths):
         """Whole sequences: x [rows, columns] with int32 offsets cu [sequences + 1] on the device; ``lengths`` int32 [sequences]
-        are those of the sequences.  Fills their pages and returns [rows, heads * d]."""
+        are those of the sequences.  Up to 65535 rows.  Fills their pages and returns [rows, heads * d]."""
         q, k, v = self._project(x)
         self._attention.cache_append(k, v, self.k_pages, self.v_pages, page_table, lengths, cu=cu)
         return self._attention.window_attention(q, k, v, cu_q=cu, **self.mask)[0].view(x.shape[0], -1)
