@@ -11,7 +11,6 @@ Five kinds of case (``case["kind"]``):
   append   new keys and values written into those pages
   q4       a few vectors times a matrix of 4-bit weights with a scale (and a zero point) per group of columns
 """
-import functools
 import importlib
 import math
 import pathlib
@@ -165,7 +164,6 @@ def prepare(case, seed):
     return st
 
 
-@functools.lru_cache
 def _package(module):
     root = str(pathlib.Path(__file__).resolve().parents[1] / "spmm-research_amd")
     if root not in sys.path:
