@@ -316,7 +316,7 @@ extern "C" int spmm_attn_window(const spmm_attn_desc_t *a, const spmm_attn_rows_
         (st = check_rows(a, v, W, "v", nb, a->k_len, a->kv_heads, false, &A.v)) ||
         (st = check_rows(a, out, W, "out", nb, a->q_len, a->heads, true, &A.out)))
         return st;
-    if (nb == 0 || a->q_len == 0 || a->batch == 0) return SPMM_HIP_OK;
+    if (nb == 0 || a->q_len == 0 || (a->batch == 0 && !a->zero_rest)) return SPMM_HIP_OK;      // no sequence: all rows lie behind it
     if (!lse || (uintptr_t)lse % 4) return fail(SPMM_HIP_ERR_ARG, "%s: lse is NULL or not aligned", W);
     A.lse = lse;
     const bool direct = A.k.direct && A.v.direct, few = (nb * a->q_len + 127) / 128 * a->heads < 128;

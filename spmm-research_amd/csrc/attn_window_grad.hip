@@ -736,7 +736,7 @@ extern "C" int spmm_attn_window_grad(const spmm_attn_desc_t *a, const spmm_attn_
         (st = check_rows(a, dk, W, "dk", nb, a->k_len, a->kv_heads, true, &A.dk)) ||
         (st = check_rows(a, dv, W, "dv", nb, a->k_len, a->kv_heads, true, &A.dv)))
         return st;
-    if (a->batch == 0) return SPMM_HIP_OK;
+    if (nb == 0 || (a->batch == 0 && !a->zero_rest)) return SPMM_HIP_OK;
     GradWork w;
     if ((st = grad_work(a, W, packed, &w))) return st;
     if (w.total > 0) {

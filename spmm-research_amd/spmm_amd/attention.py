@@ -174,8 +174,6 @@ def window_attention(q, k, v, window: int = 0, sinks: int = 0, scale: float | No
             lse = q.new_empty(q.shape[:-1], dtype=torch.float32)
         else:
             _tensor("lse", lse, torch.float32, dev, q.shape[:-1], True)
-        if packed and d.batch == 0 and d.zero_rest:
-            return out.zero_(), lse.fill_(float("-inf"))
     _check("window_attention", lib.spmm_attn_window(d, qr, kr, vr, pq, pk, _rows(out, os, packed), lse.data_ptr(), st))
     return out, lse
 
@@ -204,8 +202,6 @@ def window_attention_backward(dout, q, k, v, out, lse, window: int = 0, sinks: i
             res.append(g)
             rows.append(_rows(g, s, packed))
         work = q.new_empty(need.value, dtype=torch.uint8)
-        if packed and d.batch == 0 and d.zero_rest:
-            return tuple(g.zero_() for g in res)
     _check("window_attention_backward", lib.spmm_attn_window_grad(d, dr, qr, kr, vr, outr, lse.data_ptr(), pq, pk, *rows,
                                                                   work.data_ptr(), need.value, st))
     return tuple(res)
