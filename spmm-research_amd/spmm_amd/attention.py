@@ -160,18 +160,24 @@ def window_attention(q, k, v, window: int = 0, sinks: int = 0, scale: float | No
     q [batch, rows, heads, d], k and v [batch, key rows, key heads, d]; or, with int32 offsets ``cu_q`` and ``cu_k``
     ([sequences + 1], on the device; cu_k defaults to cu_q), [rows, heads, d] and [key rows, key heads, d].
     ``scale`` defaults to d ** -0.5.  out is like q, lse float32 with q's shape less its last dimension (the log of the sum
-    of the exponentials, -inf where a query sees nothing).  With offsets, rows behind the last sequence are set to 0
-    (lse -inf) in an out that the call allocates and left as they are, in lse too, if ``out`` is given."""
-    packed, d, pq, pk, qr, kr, vr, dev, dt = _window_operands(q, k, v, window, sinks, scale, cu_q, cu_k, out is None)
+    of the exponentials, -inf where a query sees nothing).  With offsets, rows behind the last sequence are 0 in an out and
+    -inf in an lse that the call allocates, and left as they are in one that is given."""
+    whole = out is None and lse is None
+    packed, d, pq, pk, qr, kr, vr, dev, dt = _window_operands(q, k, v, window, sinks, scale, cu_q, cu_k, whole)
+    fill = packed and not whole
     st, where = _place(dev, stream)
     with where or _HERE:
         if out is None:
             out = q.new_empty(q.shape)
             os = out.stride()
+            if fill:
+                out.zero_()
         else:
             os = _tensor("out", out, dt, dev, q.shape)
         if lse is None:
             lse = q.new_empty(q.shape[:-1], dtype=torch.float32)
+            if fill:
+                lse.fill_(float("-inf"))
         else:
             _tensor("lse", lse, torch.float32, dev, q.shape[:-1], True)
     _check("window_attention", lib.spmm_attn_window(d, qr, kr, vr, pq, pk, _rows(out, os, packed), lse.data_ptr(), st))
@@ -181,10 +187,10 @@ def window_attention(q, k, v, window: int = 0, sinks: int = 0, scale: float | No
 def window_attention_backward(dout, q, k, v, out, lse, window: int = 0, sinks: int = 0, scale: float | None = None,
                               cu_q=None, cu_k=None, dq=None, dk=None, dv=None, stream: int | None = None):
     """Gradients (dq, dk, dv) of ``window_attention`` for the gradient ``dout`` of its out; out, lse: what it returned,
-    the other arguments as they were.  With offsets, rows behind the last sequence are set to 0 if the call allocates
-    all three, and left as they are if any is given."""
-    packed, d, pq, pk, qr, kr, vr, dev, dt = _window_operands(q, k, v, window, sinks, scale, cu_q, cu_k,
-                                                              dq is None and dk is None and dv is None)
+    the other arguments as they were.  With offsets, rows behind the last sequence are 0 in gradients that the call
+    allocates and left as they are in those that are given."""
+    whole = dq is None and dk is None and dv is None
+    packed, d, pq, pk, qr, kr, vr, dev, dt = _window_operands(q, k, v, window, sinks, scale, cu_q, cu_k, whole)
     dr = _rows(dout, _tensor("dout", dout, dt, dev, q.shape), packed)
     outr = _rows(out, _tensor("out", out, dt, dev, q.shape), packed)
     _tensor("lse", lse, torch.float32, dev, q.shape[:-1], True)
@@ -197,6 +203,8 @@ def window_attention_backward(dout, q, k, v, out, lse, window: int = 0, sinks: i
             if g is None:
                 g = t.new_empty(t.shape)
                 s = g.stride()
+                if packed and not whole:
+                    g.zero_()
             else:
                 s = _tensor(name, g, dt, dev, t.shape)
             res.append(g)
