@@ -4,7 +4,8 @@ Beside ``spmm_amd.pbv`` (K = 1 products with pruned weights): here the weights a
 for every ``group`` columns of a row, ``w = scale * (q - zero)``.  ``Q4Format`` lays the weights out on the device once,
 in the order in which the product reads them; ``matvec`` multiplies.  Arguments are torch tensors on one HIP device; work
 is ordered on ``stream`` (an integer hipStream_t; by default the device's current stream) and products can be captured
-in a graph.  There is no CPU path.
+in a graph.  There is no CPU path, and no gradient: outside ``torch.no_grad()`` scales and vectors that require one are
+refused.
 """
 from __future__ import annotations
 
@@ -13,7 +14,7 @@ import ctypes as C
 import torch
 
 from . import SpmmHipError, _open
-from .attention import F16, BF16, F32, _HERE, _int, _place, _tensor
+from .attention import F16, BF16, F32, _HERE, _int, _place, _tensor, _unrecorded
 
 _DTYPES = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
 
@@ -57,6 +58,7 @@ class Q4Format:
             raise TypeError(f"scales are {scales.dtype}: float32, float16 or bfloat16")
         if len(ps) != 2 or len(ss) != 2:
             raise ValueError("packed and scales must have two dimensions")
+        _unrecorded(scales=scales)
         self.rows = packed.shape[0]
         self.cols = 2 * packed.shape[1] if cols is None else _int("cols", cols, 0)
         self.group = _int("group", group, 1)
@@ -86,6 +88,7 @@ class Q4Format:
         nd = len(xs)
         if nd not in (1, 2) or x.shape[-1] != self.cols:
             raise ValueError(f"x {tuple(x.shape)}: [{self.cols}] or [tokens, {self.cols}] expected")
+        _unrecorded(x=x)
         shape = (self.rows,) if nd == 1 else (x.shape[0], self.rows)
         st, where = _place(self._dev, stream)
         with where or _HERE:
