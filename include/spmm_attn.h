@@ -11,7 +11,8 @@
  *   s[j] = scale * <q_i, k_j>,  lse = log sum_visible exp(s),  out = sum_visible exp(s - lse) v_j
  *
  * A query that sees no key (Lk < Lq) has out = 0, lse = -inf and gradients of 0.  What stands in places that a query
- * does not see, infinities and NaN included, does not reach its results.
+ * does not see, infinities and NaN included, does not reach its results.  A value that it sees and that is not finite is
+ * added to out as it is, however small its weight.
  *
  * Query head h reads key/value head h / (heads / kv_heads).  Element types: SPMM_ATTN_F32, SPMM_ATTN_F16,
  * SPMM_ATTN_BF16; scores, softmax statistics and sums are 32-bit floats.  With the 16-bit types spmm_attn_window rounds

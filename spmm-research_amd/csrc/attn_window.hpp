@@ -80,6 +80,7 @@ __device__ __attribute__((noinline)) void careful_product(Careful<T, DP, ROWS> *
                 if (BOTH) c->acc[d] = mma32(f, low, c->acc[d]);
             }
         }
+    if (last < j0) return;
 #pragma unroll 1
     for (int rr = 0; rr < ROWS; ++rr) {
         // rows are keys and the column a query at p, or rows are queries at j0 + rr and the column key p
@@ -91,6 +92,35 @@ __device__ __attribute__((noinline)) void careful_product(Careful<T, DP, ROWS> *
                 const float x = (float)tile[Tile<T, DP>::at(rr, d * 32 + 8 * (r >> 2) + (r & 3) + 4 * (lane >> 5))];
                 if (seen && !finite_f(x)) c->acc[d][r] += x;
             }
+    }
+}
+
+// acc += the values that are not finite of the keys from `from` to `to` that the lane's query, at position p, sees; a lane has the
+// elements of a result's column that the products give it.  Without their weights: a weight is positive, but may be rounded
+// to 0, in which case a product would make NaN of an infinity.  64 lanes look a row over, eight rows on their way at a time.
+template <typename T, int DP> struct Sums {
+    f32x16 acc[DP / 32];
+};
+template <typename T, int DP>
+__device__ __attribute__((noinline)) void add_not_finite_rows(Sums<T, DP> *c, const T *v, int64_t row, int dim, int lane, Mask mask,
+                                                              int p, int from, int to) {
+#pragma unroll 1
+    for (int j0 = from; j0 <= to; j0 += 8) {
+        float x[8][2];
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+                x[i][s] = j0 + i <= to && lane + 64 * s < dim ? (float)v[(int64_t)(j0 + i) * row + lane + 64 * s] : 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+                for (unsigned long long m = __ballot(!finite_f(x[i][s])); m; m &= m - 1) {
+                    const int el = __ffsll(m) - 1, e = el + 64 * s;
+                    const float y = __shfl(x[i][s], el);
+                    if ((lane >> 5) == (e >> 2 & 1) && mask.sees(p, j0 + i)) c->acc[e >> 5][(e >> 3 & 3) * 4 + (e & 3)] += y;
+                }
     }
 }
 
