@@ -144,9 +144,9 @@ __device__ __forceinline__ void add_values(f32x4 (&o)[VE], const f32x4 &w, const
     }
 }
 
-// Values that are not finite, taken out of the pieces and added by themselves: with a weight that was rounded to 0, or as its
-// remainder is, the products would make NaN of an infinity.
-template <typename T, int VE> __device__ __forceinline__ void add_not_finite(f32x4 (&o)[VE], typename Piece<T, VE>::vec (&v)[4]) {
+// Values that are not finite, taken out of the pieces and summed by themselves in a wave's `extra`, a number a column: with a weight
+// that was rounded to 0, or as its remainder is, and in a rescaling by 0, a product would make NaN of an infinity.
+template <typename T, int VE> __device__ __forceinline__ void take_not_finite(float *extra, typename Piece<T, VE>::vec (&v)[4], int lane) {
 #pragma unroll
     for (int j = 0; j < VE; ++j) {
         float x = 0.f;
@@ -158,7 +158,7 @@ template <typename T, int VE> __device__ __forceinline__ void add_not_finite(f32
             }
         x += __shfl_xor(x, 16);
         x += __shfl_xor(x, 32);
-        o[j] += x;
+        if (lane < 16 && x != 0.f) extra[lane * VE + j] += x;
     }
 }
 
@@ -235,9 +235,12 @@ __global__ __launch_bounds__(PW * 64, paged_blocks(sizeof(T) == 2)) void paged_k
         return pg < 0 || pg >= A.pages ? -2 : pg;
     };
 
+    __shared__ float extra[PW][DP];
+#pragma unroll
+    for (int i = 0; i < DP; i += WAVE) extra[wave][i + lane] = 0.f;
     f32x4 o[VE];
     float m, sum;
-    // A second time, and with care, if some sum is NaN in the end: each wave for itself.
+    // A second time, and with care, if some sum is not finite in the end: each wave for itself.
     for (bool careful = false;; careful = true) {
 #pragma unroll
         for (int j = 0; j < VE; ++j) o[j] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -286,15 +289,15 @@ __global__ __launch_bounds__(PW * 64, paged_blocks(sizeof(T) == 2)) void paged_k
                 sc[r] = __builtin_amdgcn_exp2f(sc[r] - base);
                 sum += sc[r];
             }
-            if (careful) add_not_finite<T, VE>(o, vr);
+            if (careful) take_not_finite<T, VE>(extra[wave], vr, lane);
             add_values<T, VE>(o, sc, vr);
         }
-        bool nan = false;
+        bool odd = false;
 #pragma unroll
         for (int j = 0; j < VE; ++j)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) nan |= o[j][r] != o[j][r];
-        if (careful || !__any(nan)) break;
+            for (int r = 0; r < 4; ++r) odd |= !finite_f(o[j][r]);
+        if (careful || !__any(odd)) break;
     }
     sum += __shfl_xor(sum, 16);
     sum += __shfl_xor(sum, 32);
@@ -319,7 +322,9 @@ __global__ __launch_bounds__(PW * 64, paged_blocks(sizeof(T) == 2)) void paged_k
 #pragma unroll
         for (int w = 0; w < PW; ++w) mx = fmaxf(mx, sm[w][hh]);
         const float base = mx == -INFINITY ? 0.f : mx;
-        float tot = 0.f, acc = 0.f;
+        float tot = 0.f, acc = 0.f, x = 0.f;                // x: 0, or not finite
+#pragma unroll
+        for (int w = 0; w < PW; ++w) x += extra[w][d];
 #pragma unroll
         for (int w = 0; w < PW; ++w) {
             const float f = __builtin_amdgcn_exp2f(sm[w][hh] - base);
@@ -328,7 +333,7 @@ __global__ __launch_bounds__(PW * 64, paged_blocks(sizeof(T) == 2)) void paged_k
         }
         const int hd = kv * group + g0 + hh;
         if (parts == 1) {
-            ((T *)A.out.ptr)[b * A.out.seq + hd * A.out.head + d] = narrow<T>(tot == 0.f ? 0.f : acc / tot);
+            ((T *)A.out.ptr)[b * A.out.seq + hd * A.out.head + d] = narrow<T>((tot == 0.f ? 0.f : acc / tot) + x);
             if (d == 0) A.lse[b * A.heads + hd] = tot == 0.f ? -INFINITY : mx * LN2 + __logf(tot);
         } else {
             const int64_t at = (int64_t)hd * A.cap + id;
@@ -336,13 +341,13 @@ __global__ __launch_bounds__(PW * 64, paged_blocks(sizeof(T) == 2)) void paged_k
                 A.part[2 * at] = mx;
                 A.part[2 * at + 1] = tot;
             }
-            A.part[2 * (int64_t)A.heads * A.cap + at * A.dim + d] = acc;
+            A.part[2 * (int64_t)A.heads * A.cap + at * A.dim + d] = acc + x;
         }
     }
 }
 
 // A block a (sequence, head): its parts joined in an order that is fixed by their number.  Each of the four waves takes a
-// quarter of them, eight parts on their way at a time.
+// quarter of them, eight parts on their way at a time.  What is not finite in a part is added to the result as it is.
 constexpr int JW = 4;
 template <typename T> __global__ __launch_bounds__(JW * 64) void paged_join_kernel(PagedArgs A) {
     const int64_t x = blockIdx.x, b = x / A.heads;
@@ -356,7 +361,7 @@ template <typename T> __global__ __launch_bounds__(JW * 64) void paged_join_kern
 #pragma unroll
     for (int d = 32; d; d /= 2) mx = fmaxf(mx, __shfl_xor(mx, d));
     const float base = mx == -INFINITY ? 0.f : mx;
-    float tot = 0.f, a0 = 0.f, a1 = 0.f;
+    float tot = 0.f, a0 = 0.f, a1 = 0.f, x0 = 0.f, x1 = 0.f;
     const int e0 = min(lane, A.dim - 1), e1 = min(lane + WAVE, A.dim - 1);
     const int per = (splits + JW - 1) / JW, last = min((wave + 1) * per, splits);
     for (int s0 = wave * per; s0 < last; s0 += WAVE) {
@@ -383,15 +388,20 @@ template <typename T> __global__ __launch_bounds__(JW * 64) void paged_join_kern
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const float fs = __shfl(f, s + i);
-                a0 = s + i < n ? a0 + fs * y0[i] : a0;
-                a1 = s + i < n ? a1 + fs * y1[i] : a1;
+                const float g0 = finite_f(y0[i]) ? y0[i] : 0.f, g1 = finite_f(y1[i]) ? y1[i] : 0.f;
+                a0 += fs * g0;                              // fs is 0 past the last part
+                a1 += fs * g1;
+                x0 += y0[i] - g0;
+                x1 += y1[i] - g1;
             }
         }
     }
-    __shared__ float wt[JW], w0[JW][WAVE], w1[JW][WAVE];
+    __shared__ float wt[JW], w0[JW][WAVE], w1[JW][WAVE], wx0[JW][WAVE], wx1[JW][WAVE];
     if (lane == 0) wt[wave] = tot;
     w0[wave][lane] = a0;
     w1[wave][lane] = a1;
+    wx0[wave][lane] = x0;
+    wx1[wave][lane] = x1;
     __syncthreads();
     if (wave) return;
 #pragma unroll
@@ -399,11 +409,13 @@ template <typename T> __global__ __launch_bounds__(JW * 64) void paged_join_kern
         tot += wt[i];
         a0 += w0[i][lane];
         a1 += w1[i][lane];
+        x0 += wx0[i][lane];
+        x1 += wx1[i][lane];
     }
     const float inv = tot == 0.f ? 0.f : 1.f / tot;
     T *dst = (T *)A.out.ptr + b * A.out.seq + hd * A.out.head;
-    if (lane < A.dim) dst[lane] = narrow<T>(a0 * inv);
-    if (lane + WAVE < A.dim) dst[lane + WAVE] = narrow<T>(a1 * inv);
+    if (lane < A.dim) dst[lane] = narrow<T>(a0 * inv + x0);
+    if (lane + WAVE < A.dim) dst[lane + WAVE] = narrow<T>(a1 * inv + x1);
     if (lane == 0) A.lse[x] = tot == 0.f ? -INFINITY : mx * LN2 + __logf(tot);
 }
 

@@ -61,3 +61,44 @@ def test_window_both_signs_and_first_keys(A, dtype):
     assert out[both][..., 7].isnan().all() and (out[(i >= 3) & ~both][..., 7] == math.inf).all()
     low = (i >= 220) & (i < 310)
     assert (out[low][..., 8] == -math.inf).all() and out[~low][..., 8].isfinite().all()
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("nats", [20, 130])
+@pytest.mark.parametrize("length", [40, 250, 5000])
+def test_paged(A, dtype, nats, length):
+    h, hk, d, page = 4, 2, 64, 16
+    pages = -(-length // page)
+    k, v = (rnd(i, pages, page, hk, d, dtype=dtype) for i in (1, 2))
+    q = rnd(3, 1, h, d, dtype=dtype)
+    q[..., 0] = 4.0
+    table = torch.arange(pages, dtype=torch.int32)[None].cuda()
+    lengths = torch.tensor([length], dtype=torch.int32).cuda()
+    for where, value in ((0, math.inf), (length // 2, -math.inf), (length - 1, math.inf), (length // 3, math.nan)):
+        kk, vv = k.clone(), v.clone()
+        kk[where // page, where % page, :, 0] = -nats * d ** 0.5 / 4
+        args = (q.cuda(), kk.cuda())
+        ref, rl = A.paged_attention(*args, vv.cuda(), table, lengths)
+        vv[where // page, where % page, :, 3] = value
+        out, lse = A.paged_attention(*args, vv.cuda(), table, lengths)
+        assert is_value(out[..., 3], value), (where, value)
+        rest = [c for c in range(d) if c != 3]
+        assert torch.equal(lse, rl) and torch.isfinite(out[..., rest]).all()
+        # what the 16-bit remainders of the other weights add is the same, in the same order
+        assert torch.equal(out[..., rest], ref[..., rest])
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_paged_scores_that_rise(A, dtype):
+    """The value that is infinite comes first and the scores rise by hundreds of powers of two after it, in the same wave and
+    in others: what is rescaled stays infinite."""
+    length, page, d = 400, 16, 64
+    k, v = (rnd(i, 25, page, 1, d, dtype=dtype) for i in (1, 2))
+    k[..., 0] = torch.arange(400).reshape(25, page, 1).float().mul(4).to(dtype)
+    q = torch.zeros(1, 2, d, dtype=dtype)
+    q[..., 0] = 4.0
+    v[0, 5, 0, 9] = math.inf
+    table = torch.arange(25, dtype=torch.int32)[None].cuda()
+    for n in (100, 250, 400):
+        out, lse = A.paged_attention(q.cuda(), k.cuda(), v.cuda(), table, torch.tensor([n], dtype=torch.int32).cuda())
+        assert (out[..., 9] == math.inf).all() and torch.isfinite(out[..., :9]).all() and torch.isfinite(lse).all()
