@@ -90,8 +90,8 @@ def _tensor(name: str, t, dtype=None, device: int | None = None, shape=None, con
     return s
 
 
-def _unrecorded(**operands) -> None:
-    """None of them needs a gradient that the call would lose."""
+def _lost(**operands) -> None:
+    """Refuses operands whose gradient a call would lose."""
     for name, t in operands.items():
         if t.requires_grad and torch.is_grad_enabled():
             raise ValueError(f"{name} requires a gradient, which this call would lose: call it under torch.no_grad(), or in "
@@ -176,7 +176,8 @@ def window_attention(q, k, v, window: int = 0, sinks: int = 0, scale: float | No
     -inf in an lse that the call allocates, and left as they are in one that is given."""
     whole = out is None and lse is None
     packed, d, pq, pk, qr, kr, vr, dev, dt = _window_operands(q, k, v, window, sinks, scale, cu_q, cu_k, whole)
-    _unrecorded(q=q, k=k, v=v)
+    if q.requires_grad or k.requires_grad or v.requires_grad:
+        _lost(q=q, k=k, v=v)
     fill = packed and not whole
     st, where = _place(dev, stream)
     with where or _HERE:
@@ -205,7 +206,8 @@ def window_attention_backward(dout, q, k, v, out, lse, window: int = 0, sinks: i
     whole = dq is None and dk is None and dv is None
     packed, d, pq, pk, qr, kr, vr, dev, dt = _window_operands(q, k, v, window, sinks, scale, cu_q, cu_k, whole)
     dr = _rows(dout, _tensor("dout", dout, dt, dev, q.shape), packed)
-    _unrecorded(dout=dout, q=q, k=k, v=v)
+    if dout.requires_grad or q.requires_grad or k.requires_grad or v.requires_grad:
+        _lost(dout=dout, q=q, k=k, v=v)
     outr = _rows(out, _tensor("out", out, dt, dev, q.shape), packed)
     _tensor("lse", lse, torch.float32, dev, q.shape[:-1], True)
     st, where = _place(dev, stream)
@@ -260,7 +262,8 @@ def paged_attention(q, k_pages, v_pages, page_table, lengths, window: int = 0, s
         raise ValueError(f"q {tuple(q.shape)}: [batch, heads, d] expected")
     dev, dt, batch = q.get_device(), q.dtype, q.shape[0]
     pages = _pages(k_pages, v_pages, page_table, lengths, q.shape[2], dt, dev, batch)
-    _unrecorded(q=q, k_pages=k_pages, v_pages=v_pages)
+    if q.requires_grad or k_pages.requires_grad or v_pages.requires_grad:
+        _lost(q=q, k_pages=k_pages, v_pages=v_pages)
     d = _desc(q, dev, k_pages.shape[2], window, sinks, scale, batch, 1, 0)
     room = min(pages.table_cols * pages.page_rows, 2 ** 30 - 1)
     longest = room if max_length is None else min(_int("max_length", max_length, 0), room)
@@ -305,6 +308,7 @@ def cache_append(k, v, k_pages, v_pages, page_table, lengths, cu=None, stream: i
     pages = _pages(k_pages, v_pages, page_table, lengths, dim, dt, dev, batch)
     if k_pages.shape[2] != heads:
         raise ValueError(f"{heads} key heads, the pages have {k_pages.shape[2]}")
-    _unrecorded(k=k, v=v, k_pages=k_pages, v_pages=v_pages)
+    if k.requires_grad or v.requires_grad or k_pages.requires_grad or v_pages.requires_grad:
+        _lost(k=k, v=v, k_pages=k_pages, v_pages=v_pages)
     _check("cache_append", lib.spmm_attn_append(_desc(k, dev, heads, 0, 0, 1.0, batch, rows, 0), _rows(k, ks, True),
                                                 _rows(v, vs, True), pc, pages, _place(dev, stream)[0]))

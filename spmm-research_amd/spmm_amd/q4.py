@@ -14,7 +14,7 @@ import ctypes as C
 import torch
 
 from . import SpmmHipError, _open
-from .attention import F16, BF16, F32, _HERE, _int, _place, _tensor, _unrecorded
+from .attention import F16, BF16, F32, _HERE, _int, _place, _tensor, _lost
 
 _DTYPES = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
 
@@ -58,7 +58,8 @@ class Q4Format:
             raise TypeError(f"scales are {scales.dtype}: float32, float16 or bfloat16")
         if len(ps) != 2 or len(ss) != 2:
             raise ValueError("packed and scales must have two dimensions")
-        _unrecorded(scales=scales)
+        if scales.requires_grad:
+            _lost(scales=scales)
         self.rows = packed.shape[0]
         self.cols = 2 * packed.shape[1] if cols is None else _int("cols", cols, 0)
         self.group = _int("group", group, 1)
@@ -88,7 +89,8 @@ class Q4Format:
         nd = len(xs)
         if nd not in (1, 2) or x.shape[-1] != self.cols:
             raise ValueError(f"x {tuple(x.shape)}: [{self.cols}] or [tokens, {self.cols}] expected")
-        _unrecorded(x=x)
+        if x.requires_grad:
+            _lost(x=x)
         shape = (self.rows,) if nd == 1 else (x.shape[0], self.rows)
         st, where = _place(self._dev, stream)
         with where or _HERE:
