@@ -116,9 +116,14 @@ def _place(device: int, stream):
     """(stream handle, context in which allocations belong to that stream, None where they do already)."""
     if stream is None:
         return torch._C._cuda_getCurrentRawStream(device), None
+    return stream, torch.cuda.stream(_stream(device, stream))
+
+
+def _stream(device: int, stream: int):
+    """torch's stream of that handle.  0 is the null stream, of which ExternalStream would make a new one."""
     if isinstance(stream, bool) or not isinstance(stream, int):
         raise TypeError("stream must be an integer hipStream_t")
-    return stream, torch.cuda.stream(torch.cuda.ExternalStream(stream, device=device))
+    return torch.cuda.ExternalStream(stream, device=device) if stream else torch.cuda.default_stream(device)
 
 
 _HERE = contextlib.nullcontext()
