@@ -188,8 +188,13 @@ class TokenPipeline:
         self.mask = dict(window=window, sinks=sinks, scale=scale)
         self.k_pages, self.v_pages = (torch.zeros(pages, page_rows, kv_heads, self.dim, dtype=w_q.dtype, device=w_q.device)
                                       for _ in range(2))
+        self._stream = attention._place(w_q.device.index, None)[0]
 
     def _project(self, x):
+        stream = self._attention._place(self.k_pages.get_device(), None)[0]
+        if stream != self._stream:                       # the pages outlive this call's work if the pipeline is dropped
+            for t in (self.k_pages, self.v_pages):
+                t.record_stream(self._attention._stream(self.k_pages.get_device(), stream))
         return (self.w[t].matvec(x).view(x.shape[0], n, self.dim) for t, n in
                 (("Q", self.heads), ("K", self.kv_heads), ("V", self.kv_heads)))
 

@@ -14,7 +14,7 @@ import ctypes as C
 import torch
 
 from . import SpmmHipError, _open
-from .attention import F16, BF16, F32, _HERE, _int, _place, _tensor, _lost
+from .attention import F16, BF16, F32, _HERE, _int, _lost, _place, _stream, _tensor
 
 _DTYPES = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
 
@@ -46,7 +46,8 @@ class Q4Format:
 
     packed uint8 [rows, (cols + 1) // 2], column 2 i in the low half of byte i; scales [rows, groups], float32, float16 or
     bfloat16 (the type of the vectors too), groups = cols / group rounded up; zeros uint8 [rows, groups], or None for
-    8.  group: 32, 64 or a multiple of 128.  The arguments are not kept; changing them afterwards changes nothing."""
+    8.  group: 32, 64 or a multiple of 128.  The arguments are not kept; what is written to them on ``stream``, or after it, changes
+    nothing."""
 
     format_name = "HIP_Q4_MI355X"
 
@@ -76,6 +77,10 @@ class Q4Format:
         st, where = _place(dev, stream)
         with where or _HERE:
             self._layout = torch.empty(need.value, dtype=torch.uint8, device=packed.device)
+        self._stream = st
+        if where is not None:                            # the memory of what is read is not handed on before that is done
+            for t in (packed, scales) if zeros is None else (packed, scales, zeros):
+                t.record_stream(_stream(dev, st))
         self.mem_footprint = float(need.value)
         _check("Q4Format", lib.spmm_q4_layout(self._d, packed.data_ptr(), ps[0], scales.data_ptr(), ss[0],
                                               zeros.data_ptr() if zeros is not None else None, zs[0],
@@ -84,7 +89,7 @@ class Q4Format:
     def matvec(self, x, out=None, stream: int | None = None):
         """x W^T: x [cols] or [tokens, cols] (rows any distance apart) -> [rows] or [tokens, rows].  Made for a few
         vectors: every 16 of them (5 in float32) read the weights once more.  A call on another stream than the one the
-        format was made on has to come after it."""
+        format was made on has to come after it; the format may be dropped as soon as the call returns."""
         xs = _tensor("x", x, self.dtype, self._dev)
         nd = len(xs)
         if nd not in (1, 2) or x.shape[-1] != self.cols:
@@ -101,6 +106,8 @@ class Q4Format:
                 os = _tensor("out", out, self.dtype, self._dev, shape)
             if self.cols == 0:
                 return out.zero_()
+        if st != self._stream:                           # the layout, which no caller has, outlives the product there
+            self._layout.record_stream(_stream(self._dev, st))
         _check("matvec", lib.spmm_q4_matvec(self._d, self._layout.data_ptr(), x.data_ptr(), xs[0] if nd == 2 else 0,
                                             x.shape[0] if nd == 2 else 1, out.data_ptr(), os[0] if nd == 2 else self.rows, st))
         return out
