@@ -203,7 +203,7 @@ class TokenPipeline:
         are those of the sequences.  Up to 65535 rows.  Fills their pages and returns [rows, heads * d]."""
         q, k, v = self._project(x)
         self._attention.cache_append(k, v, self.k_pages, self.v_pages, page_table, lengths, cu=cu)
-        return self._attention.window_attention(q, k, v, cu_q=cu, **self.mask)[0].view(x.shape[0], -1)
+        return self._attention.window_attention(q, k, v, cu_q=cu, **self.mask)[0].view(x.shape[0], self.heads * self.dim)
 
     def step(self, x, page_table, lengths, max_length: int | None = None):
         """One new token a sequence: x [sequences, columns], ``lengths`` with the new token counted.  Adds it to the cache
@@ -211,4 +211,4 @@ class TokenPipeline:
         q, k, v = self._project(x)
         self._attention.cache_append(k, v, self.k_pages, self.v_pages, page_table, lengths)
         return self._attention.paged_attention(q, self.k_pages, self.v_pages, page_table, lengths, max_length=max_length,
-                                               **self.mask)[0].view(x.shape[0], -1)
+                                               **self.mask)[0].view(x.shape[0], self.heads * self.dim)
