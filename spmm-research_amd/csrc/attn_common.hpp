@@ -129,7 +129,10 @@ template <typename T, int DP> struct Tile {
 // wave's but the last n are there) and a barrier, and a wave has waited for all before it ends.  (With the builtin
 // it does count them, and waits for every one of them before the next transposing read of any tile.)
 // m0 says where in LDS; a load may read it one wait state after it is written, and scalar registers that a vector
-// instruction wrote (readfirstlane) five after that.  The compiler does not look into the text, so the text waits.
+// instruction wrote (readfirstlane) five after that.  The compiler does not look into the text, so the text waits, and names m0
+// as written.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"          // that m0 is the compiler's own: it is named for the order with its uses
 struct Buffer {
     typedef int i32x4 __attribute__((ext_vector_type(4)));
     i32x4 rsrc;
@@ -140,12 +143,13 @@ struct Buffer {
     // where in LDS: the low half of the address
     static __device__ __forceinline__ int place(const void *tile) { return uniform((int)(uint32_t)(uintptr_t)tile); }
     __device__ __forceinline__ void to_lds16(void *tile, int off) const {
-        asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(place(tile)), "v"(off), "s"(rsrc) : "memory");
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(place(tile)), "v"(off), "s"(rsrc) : "memory", "m0");
     }
     __device__ __forceinline__ void to_lds4(void *tile, int off) const {
-        asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(place(tile)), "v"(off), "s"(rsrc) : "memory");
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(place(tile)), "v"(off), "s"(rsrc) : "memory", "m0");
     }
 };
+#pragma clang diagnostic pop
 template <int LEFT = 0> __device__ __forceinline__ void arrived() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LEFT) : "memory"); }
 
 // Brings the R rows of a tile from memory to LDS, THREADS threads together.
