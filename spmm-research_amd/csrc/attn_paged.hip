@@ -70,11 +70,17 @@ __device__ __forceinline__ int parts_of(int tiles, int per) {
 }
 // first: tiles of sequence `lane`
 __device__ __forceinline__ int plan(const PagedArgs &A, int lane, int first) {
-    if (A.batch <= WAVE) {                                  // the tiles of 64 sequences are less than 2^32
-        uint32_t total = first;
+    if (A.batch <= WAVE) {
+        // A sequence has 2^26 tiles and a few at most: the sum of 64 takes more than 32 bits, and with 2^27 a part none is cut.
+        uint32_t low = first & 0xffff, high = (uint32_t)first >> 16;
 #pragma unroll
-        for (int d = 32; d; d /= 2) total += __shfl_xor(total, d);
-        const int lo = max(SPLIT_MIN / PK, (int)((uint32_t)uniform((int)total) / (uint32_t)A.room) + 1);
+        for (int d = 32; d; d /= 2) {
+            low += __shfl_xor(low, d);
+            high += __shfl_xor(high, d);
+        }
+        const uint64_t total = ((uint64_t)(uint32_t)uniform((int)high) << 16) + (uint32_t)uniform((int)low);
+        const uint64_t each = total >> 32 ? total / (uint32_t)A.room : (uint32_t)total / (uint32_t)A.room;
+        const int lo = max(SPLIT_MIN / PK, (int)min(each, (uint64_t)1 << 27) + 1);
         auto fits = [&](int per) {
             const int n = lane < A.batch ? parts_of(first, per) : 0;      // 256 at most
             int sum = 0;
