@@ -50,7 +50,7 @@ typedef struct spmm_attn_desc {
     int32_t heads, kv_heads;      /* heads a multiple of kv_heads                                               */
     int32_t dim;                  /* head width, 1 .. SPMM_ATTN_MAX_DIM                                         */
     int32_t window, sinks;        /* window 0: no limit                                                         */
-    float scale;                  /* finite                                                                     */
+    float scale;                  /* times log2(e) finite                                                       */
     int64_t batch;                /* sequences                                                                  */
     int64_t q_len, k_len;         /* without offsets: rows of every sequence; with offsets: rows of the buffers */
     int32_t zero_rest;            /* with offsets: 1 = rows behind the last sequence are set to 0 in what the

@@ -25,7 +25,8 @@ int check_desc(const spmm_attn_desc_t *a, const char *where) {
         return fail(SPMM_HIP_ERR_ARG, "%s: head width %d is not in 1 .. %d", where, a->dim, SPMM_ATTN_MAX_DIM);
     if (a->window < 0 || a->sinks < 0)
         return fail(SPMM_HIP_ERR_ARG, "%s: window %d, sinks %d", where, a->window, a->sinks);
-    if (!std::isfinite(a->scale)) return fail(SPMM_HIP_ERR_ARG, "%s: the scale is not finite", where);
+    if (!std::isfinite(a->scale * LOG2E))            // what the kernels use
+        return fail(SPMM_HIP_ERR_ARG, "%s: the scale %g, times log2(e), is not finite", where, a->scale);
     if (a->zero_rest < 0 || a->zero_rest > 1 || a->reserved != 0)
         return fail(SPMM_HIP_ERR_ARG, "%s: zero_rest %d, reserved %d", where, a->zero_rest, a->reserved);
     if (a->batch < 0 || a->q_len < 0 || a->k_len < 0)
