@@ -315,7 +315,7 @@ template <typename T, bool ZEROS, int RT> const void *matvec_sg(int group) {
            : group == 64 ? (const void *)matvec_kernel<T, ZEROS, RT, 2> : (const void *)matvec_kernel<T, ZEROS, RT, 4>;
 }
 template <typename T, bool ZEROS> const void *matvec_rt(int rt, int group) {
-    return rt == 4 ? matvec_sg<T, ZEROS, 4>(group) : rt == 2 ? matvec_sg<T, ZEROS, 2>(group) : matvec_sg<T, ZEROS, 1>(group);
+    return rt == 4 ? (const void *)matvec_kernel<T, ZEROS, 4, 1> : rt == 2 ? matvec_sg<T, ZEROS, 2>(group) : matvec_sg<T, ZEROS, 1>(group);
 }
 template <typename T> const void *matvec_of(bool zeros, int rt, int group) {
     return zeros ? matvec_rt<T, true>(rt, group) : matvec_rt<T, false>(rt, group);
@@ -408,8 +408,10 @@ int spmm_q4_matvec(const spmm_q4_desc_t *w, const void *layout, const void *x, i
     // Row tiles that share a block's x: as many as leave a block for every compute unit.  Waves that share the columns: 16 a
     // compute unit in all, one column tile each at least.  Four vectors in bf16 with 1, 2 and 4 row tiles: 4096 x 4096 weights
     // 5.8, 7.0, 10.2 us, 8192 x 8192 16.1, 12.6, 17.0, 32768 x 4096 28.6, 20.0, 18.0; 16384 x 4096 with 1024, 2048, 4096 and
-    // 8192 waves 24.1, 15.7, 12.1, 14.0.
-    const int rt = s.row_tiles >= 8 * 256 ? 4 : s.row_tiles >= 2 * 256 ? 2 : 1;
+    // 8192 waves 24.1, 15.7, 12.1, 14.0.  Four only where a tile has one scale a row: with more the registers do not hold
+    // them.  32768 x 4096, four vectors, two and four row tiles: groups of 128 in bf16 17.7, 16.3, fp16 17.6, 16.4, fp32 42.4,
+    // 33.6; of 64 19.5, 20.1, 19.2, 21.7, 44.7, 52.3; of 32 24.5, 32.8, 22.8, 35.1, 47.5, 105.9.
+    const int rt = s.row_tiles >= 8 * 256 && w->group >= 128 ? 4 : s.row_tiles >= 2 * 256 ? 2 : 1;
     const int64_t blocks = (s.row_tiles + rt - 1) / rt;
     int waves = 1;
     while (waves < WMAX && waves < A.tiles && blocks * waves < 4096) waves *= 2;
