@@ -88,8 +88,9 @@ int spmm_attn_window(const spmm_attn_desc_t *a, const spmm_attn_rows_t *q, const
                      const spmm_attn_rows_t *v, const int32_t *cu_q, const int32_t *cu_k, const spmm_attn_rows_t *out,
                      float *lse, void *stream);
 
-/* Its gradients: dout with the forward pass's out and lse -> dq, dk, dv.  `work`: spmm_attn_window_work bytes
- * (packed: 1 = the call gives offsets), 16-byte aligned. */
+/* Its gradients: dout with the forward pass's out and lse -> dq, dk, dv.  out and lse have to be what spmm_attn_window gave for
+ * just these keys, not joined over further ones: that every query's row of score gradients sums to 0 is used to take the
+ * rounding of out from dk.  `work`: spmm_attn_window_work bytes (packed: 1 = the call gives offsets), 16-byte aligned. */
 int spmm_attn_window_work(const spmm_attn_desc_t *a, int32_t packed, size_t *bytes);
 int spmm_attn_window_grad(const spmm_attn_desc_t *a, const spmm_attn_rows_t *dout, const spmm_attn_rows_t *q,
                           const spmm_attn_rows_t *k, const spmm_attn_rows_t *v, const spmm_attn_rows_t *out,

@@ -6,8 +6,9 @@
  *
  * q: 4-bit numbers 0 .. 15; zero: 8 without zero points.  x, y and the scales have one element type: SPMM_Q4_F32,
  * SPMM_Q4_F16 or SPMM_Q4_BF16.  Weights enter the products exactly (q + 16 in 16 bits), x as it is (32-bit x as three
- * 16-bit parts that sum to it); sums are 32-bit floats in a fixed order, and y is rounded once.  An infinite x, and
- * 32-bit x of more than 1e37, give NaN: the products are formed with 16 + q and 16 + zero, and those are subtracted.
+ * 16-bit parts that sum to it); sums are 32-bit floats in a fixed order, and y is rounded once.  The products are formed with
+ * 16 + q and 16 + zero over up to 128 columns at a time, and those are subtracted: an infinite x gives NaN, and so may finite
+ * ones of which such a sum, up to 31 times that of x, passes 32-bit floats (from 1.1e37 in one column, 8.5e34 in 128, on).
  *
  * The weights are laid out once (spmm_q4_layout) in the order in which the product's waves read them; the product reads
  * only the layout.  Every pointer is a device address on `device`, y does not overlap what is read, calls are ordered on `stream`, hold no state and

@@ -11,9 +11,14 @@
 // Layouts as in the forward kernel: a product's result is the next product's operand in registers.
 //
 // Bound: matrix instructions, exponentials and the reads of LDS that feed them.  Two sequences of 8192 and 8000 tokens, 32
-// heads over 8 of 128 in bf16, window 1024, 4 first keys: delta 51 us (the bytes of out and dout), grad_q 602, grad_kv 795,
-// join 15; with the forward pass 1750 us, 510 TFLOP/s of the seven products that the formulas need.  Keeping V's
-// fragments in registers as well, or two half tiles in turn, spills and is slower (2455 and 2300 us).
+// heads over 8 of 128 in bf16, window 1024, 4 first keys: 1720 to 1775 us with the forward pass, 505 to 520 TFLOP/s of the seven
+// products that the formulas need, of ten that are made.  In a trace, which slows them by a tenth, the means are delta 53 us
+// (the bytes of out and dout), grad_q 625, grad_kv 827, join 17, forward 407; matrix units busy for 46 (grad_q) and 34 %
+// (grad_kv) of the cycles, vector units for 46 and 29, LDS for 18 and 27.  Keeping V's fragments in registers as well, or two
+// half tiles in turn, spills and is slower (2455 and 2300 us).
+//
+// 257 tokens, 4 heads over 2 of 64 in 32 bits: grad_kv 39 us, grad_q 21, forward 19, join 5, delta 4, in all 84: eighteen blocks of
+// keys and a few more on 256 compute units, each of which walks its tiles in turn.
 #include "attn_window.hpp"
 
 namespace attn {
@@ -690,7 +695,7 @@ static int grad_work(const spmm_attn_desc_t *a, const char *where, bool packed, 
     const int64_t span = ((int64_t)a->window + 128 + 63) / 64 * 64;         // queries of an ordinary block of 128 keys
     // Where a sequence is longer than that, its first keys have queries beyond (2048 tokens under a window of 1024 with parts:
     // 152 us, without: 218; 257 tokens under one of 100 in 32 bits: 84 and 91); a mean of the lengths, as the offsets are not
-    // known here.
+    // known here, so a long sequence among many short ones is not split (4096 tokens alone: 421 us for 175), right but slower.
     const int64_t mean = packed && a->batch ? a->q_len / a->batch : a->q_len;
     if (a->window > 0 && a->window < a->k_len && a->sinks > 0 && a->sinks <= 128 && a->k_len > a->sinks && mean > span) {
         w->chunk = CHUNK;

@@ -205,8 +205,8 @@ def window_attention(q, k, v, window: int = 0, sinks: int = 0, scale: float | No
 
 def window_attention_backward(dout, q, k, v, out, lse, window: int = 0, sinks: int = 0, scale: float | None = None,
                               cu_q=None, cu_k=None, dq=None, dk=None, dv=None, stream: int | None = None):
-    """Gradients (dq, dk, dv) of ``window_attention`` for the gradient ``dout`` of its out; out, lse: what it returned,
-    the other arguments as they were.  With offsets, rows behind the last sequence are 0 in gradients that the call
+    """Gradients (dq, dk, dv) of ``window_attention`` for the gradient ``dout`` of its out; out, lse: what it returned
+    (for these keys, not joined with others'), the other arguments as they were.  With offsets, rows behind the last sequence are 0 in gradients that the call
     allocates and left as they are in those that are given."""
     whole = dq is None and dk is None and dv is None
     packed, d, pq, pk, qr, kr, vr, dev, dt = _window_operands(q, k, v, window, sinks, scale, cu_q, cu_k, whole)
