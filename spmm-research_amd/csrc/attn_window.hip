@@ -8,7 +8,8 @@
 //
 // A value that is not finite, if it is seen, is added to the result as it is: the block starts over, leaves such values out of
 // the products, and adds them at the end.  That none stands where it would show costs a look at the sums and a barrier a
-// block: 8192 tokens, window 1024, 32 heads over 8 of 128 in bf16 190 us from 188.
+// block: 8192 tokens, window 1024, 32 heads over 8 of 128 in bf16 190 us from 188.  With an infinity that all see, 16384 tokens
+// under a window of 2048 take 15.5 ms, and 4.0 with one in the middle.
 //
 // The weights of 16-bit types are rounded to the type for the second product, at most 2^-8 (bf16) or 2^-11 (fp16) of each,
 // as the values are; their sum is taken before that, in 32 bits.  The result's error against float64 is then 1.4 (bf16) and 1.2
@@ -211,7 +212,8 @@ __global__ __launch_bounds__(64 * MG * PG, sizeof(T) == 2 && PG == 1 ? 2 : 1) vo
         for (int d = 0; d < ND; ++d)
 #pragma unroll
             for (int r = 0; r < 16; ++r) zero = __builtin_fmaf(o[d][r], 0.f, zero);
-        if (zero != 0.f) odd[0] = 1;                 // it is 0: no tile has left with it set
+        // Not where the query's weights are NaN: its result is then.  odd[0] is 0: no tile has left with it set.
+        if (zero != 0.f && finite_f(sum + __shfl_xor(sum, 32)) && mine) odd[0] = 1;
         __syncthreads();
         careful = uniform(odd[0]);
     }
