@@ -61,6 +61,11 @@ template <typename T> __device__ __forceinline__ T *uniform(T *p) {
 // Round to nearest even; the only narrowing in these kernels apart from the stores of results.
 template <typename T> __device__ __forceinline__ T narrow(float x) { return (T)x; }
 
+// float16 has normal numbers down to 2^-14 only, and a thousand weights below that next to the largest may make up a result
+// (a first key with a high score and a value near 0 is not rare), so weights are formed as a multiple of themselves that its range
+// has room for: 2^UP<T>(top) if the largest is 2^top.  The power is taken out with the sum of the weights, at no cost.
+template <typename T> __host__ __device__ constexpr float UP(int top) { return std::is_same<T, _Float16>::value ? 15.f - top : 0.f; }
+
 // One bit per 16-bit half (or the top bit of a word) set where the exponent is all ones.
 template <typename T> __device__ __forceinline__ uint32_t not_finite(uint32_t w);
 template <> __device__ __forceinline__ uint32_t not_finite<__bf16>(uint32_t w) {

@@ -173,6 +173,7 @@ template <typename T, int DP>
 __global__ __launch_bounds__(PW * 64, paged_blocks(sizeof(T) == 2)) void paged_kernel(PagedArgs A) {
     // a lane's columns of the values: VE from VE (lane % 16) on
     constexpr int NS = DP / 32, VE = DP / 16;
+    constexpr float LIFT = UP<T>(0);                        // weights and their sums are 2^LIFT times as large
     const int group = A.heads / A.kv_heads, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, h4 = lane >> 4;
     const int hb = (group + 15) / 16;                       // blocks of 16 query heads of a group
     int id = (int)blockIdx.x;
@@ -293,7 +294,7 @@ __global__ __launch_bounds__(PW * 64, paged_blocks(sizeof(T) == 2)) void paged_k
             }
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                sc[r] = __builtin_amdgcn_exp2f(sc[r] - base);
+                sc[r] = __builtin_amdgcn_exp2f(sc[r] - (base - LIFT));
                 sum += sc[r];
             }
             if (careful) take_not_finite<T, VE>(extra[wave], vr, lane);
@@ -341,7 +342,7 @@ __global__ __launch_bounds__(PW * 64, paged_blocks(sizeof(T) == 2)) void paged_k
         const int hd = kv * group + g0 + hh;
         if (parts == 1) {
             ((T *)A.out.ptr)[b * A.out.seq + hd * A.out.head + d] = narrow<T>((tot == 0.f ? 0.f : acc / tot) + x);
-            if (d == 0) A.lse[b * A.heads + hd] = tot == 0.f ? -INFINITY : mx * LN2 + __logf(tot);
+            if (d == 0) A.lse[b * A.heads + hd] = tot == 0.f ? -INFINITY : (mx - LIFT) * LN2 + __logf(tot);
         } else {
             const int64_t at = (int64_t)hd * A.cap + id;
             if (d == 0) {
@@ -423,7 +424,7 @@ template <typename T> __global__ __launch_bounds__(JW * 64) void paged_join_kern
     T *dst = (T *)A.out.ptr + b * A.out.seq + hd * A.out.head;
     if (lane < A.dim) dst[lane] = narrow<T>(a0 * inv + x0);
     if (lane + WAVE < A.dim) dst[lane + WAVE] = narrow<T>(a1 * inv + x1);
-    if (lane == 0) A.lse[x] = tot == 0.f ? -INFINITY : mx * LN2 + __logf(tot);
+    if (lane == 0) A.lse[x] = tot == 0.f ? -INFINITY : (mx - UP<T>(0)) * LN2 + __logf(tot);
 }
 
 // ------------------------------------------------------------------------------------------------ append

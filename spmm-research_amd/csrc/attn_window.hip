@@ -32,13 +32,14 @@ namespace attn {
 template <typename T, int DP, int MG, int PG, int SUB> struct WindowShape {
     static constexpr int ROWS = 32 * MG, BN = 32 * PG * SUB, THREADS = 64 * MG * PG;
 };
-constexpr float SLACK = 8.f;
+constexpr int SLACK = 8;
 
 template <typename T, int DP, int MG, int PG, int SUB, bool DIRECT>
 __global__ __launch_bounds__(64 * MG * PG, sizeof(T) == 2 && PG == 1 ? 2 : 1) void window_kernel(WindowArgs A) {
     using L = Tile<T, DP>;
     using S = WindowShape<T, DP, MG, PG, SUB>;
     constexpr int BM = S::ROWS, BN = S::BN, THREADS = S::THREADS, ND = DP / 32, NS = DP / 16, NK = SUB;
+    constexpr float LIFT = UP<T>(SLACK);             // weights and their sum are 2^LIFT times as large
     __shared__ __align__(16) T sk[2][BN * L::PITCH], sv[2][BN * L::PITCH];
     __shared__ float sm[PG > 1 ? PG * MG * 32 : 1];  // the parts' maxima
     __shared__ int odd[2];                           // a value of the partly seen tile in this pair is not finite
@@ -152,7 +153,7 @@ __global__ __launch_bounds__(64 * MG * PG, sizeof(T) == 2 && PG == 1 ? 2 : 1) vo
             for (int d = 0; d < ND; ++d) o[d] *= alpha;
             m = top;
         }
-        const float base = m == -INFINITY ? 0.f : m;
+        const float base = (m == -INFINITY ? 0.f : m) - LIFT;
 #pragma unroll
         for (int n = 0; n < NK; ++n)
 #pragma unroll
@@ -280,7 +281,7 @@ __global__ __launch_bounds__(64 * MG * PG, sizeof(T) == 2 && PG == 1 ? 2 : 1) vo
                       f32x4{o[d][r], o[d][r + 1], o[d][r + 2], o[d][r + 3]});
     if (h == 0) {
         const int64_t row = packed ? s.q0 + i : s.b * A.q_len + i;
-        A.lse[row * A.heads + head] = sum == 0.f ? -INFINITY : m * LN2 + __logf(sum);
+        A.lse[row * A.heads + head] = sum == 0.f ? -INFINITY : (m - LIFT) * LN2 + __logf(sum);
     }
 }
 
