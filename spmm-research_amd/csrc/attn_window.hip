@@ -22,7 +22,7 @@
 // are busy for 40 % of the cycles, the vector units for 46, LDS for 21.  128 queries a block: with 256 (eight waves) 699 to
 // 728 us.  Loading the next tile's fragments ahead, unrolling by two tiles and raised wave priority gained nothing.  A ragged
 // batch of eight of 0 to 2051 tokens, 16 heads over 4 of 80, window 256: 38 us, with 64 queries a block 41 to 48; its 560 blocks
-// of up to eight tiles each meet 512 places, so 48 run in a second round.
+// of up to eight tiles each meet 512 places, so 48 run after the others.
 #include "attn_window.hpp"
 
 namespace attn {
