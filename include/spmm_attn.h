@@ -18,7 +18,7 @@
  * SPMM_ATTN_BF16; scores, softmax statistics and sums are 32-bit floats.  With the 16-bit types spmm_attn_window rounds
  * the weights to that type before they enter a product, and spmm_attn_window_grad the weights and their gradients where
  * they enter dv and dk; in dq and in spmm_attn_paged they enter as a rounded value plus its rounded remainder.  What is rounded
- * to float16 in spmm_attn_window_grad is scaled by powers of two first, so gradients small or large keep its bits.  Results
+ * to float16 is scaled by powers of two first, so small weights, and gradients small or large, keep its bits.  Results
  * do not depend on anything but the arguments: no atomics, fixed orders of summation (in spmm_attn_paged the order is
  * a matter of all the lengths).
  *
